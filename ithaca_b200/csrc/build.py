@@ -165,6 +165,18 @@ def attention_module(head_dim: int, slopes: bool = False, one_row: bool = False)
     return f"ithaca_attn{'_slopes' if slopes else ''}{'_onerow' if one_row else ''}_hd{head_dim}", ["attention_bf16.cu"], defines
 
 
+def shared_module(head_dim: int) -> tuple:
+    """Name, sources and defines of the module of a head size for sequences that share pages."""
+    return f"ithaca_attn_shared_hd{head_dim}", ["attention_shared.cu"], [f"IK_HD={head_dim}"]
+
+
+SEARCH_SOURCES = ["beam_select.cu", "copy_rows.cu"]         # what only a search over beams and forked sequences need
+
+
+def search() -> ctypes.CDLL:
+    return load_library("ithaca_search", SEARCH_SOURCES)
+
+
 PAIRS_SOURCE = "gemm_tcgen05_mc.cu"        # the pair mode of the tcgen05 product: a library of its own, optional
 
 
@@ -177,11 +189,13 @@ def pairs() -> ctypes.CDLL:
 
 
 def build_all() -> None:
-    """Everything that can be compiled ahead of time: the core library, the attention module of
+    """Everything that can be compiled ahead of time: the core library, the search library, the attention modules of
     every usual head size, and the pair mode of the tcgen05 product where its source is there."""
     core()
+    build_library("ithaca_search", SEARCH_SOURCES)
     for hd in ATTENTION_HEAD_SIZES:
         build_library(*attention_module(hd))
+        build_library(*shared_module(hd))
     for options in ATTENTION_OPTION_MODULES:
         build_library(*attention_module(*options))
     if pairs_available():

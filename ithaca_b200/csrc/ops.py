@@ -9,6 +9,7 @@ import ctypes
 import os
 from typing import Optional
 
+import numpy as np
 import torch
 
 from . import build
@@ -1222,6 +1223,142 @@ def sample(logits: torch.Tensor, temperature: float, top_k: int, top_p: float, r
                            repetition_penalty, _ptr(recent), n_recent, seed & 0xFFFFFFFFFFFFFFFF, _ptr(streams),
                            _ptr(counters), _stream()), "sample")
     return out
+
+
+# ---------------------------------------------------------------------------------------------
+# Search over beams, and what forked sequences need
+_search = None
+
+
+def _search_lib():
+    """The kernels of searches and forks: a library of its own, built and loaded by the first call that needs it."""
+    global _search
+    if _search is None:
+        l = build.search()
+        l.ik_beam_select_scratch.argtypes, l.ik_beam_select_scratch.restype = [_i, _i, _i, _i], ctypes.c_longlong
+        l.ik_beam_select.argtypes, l.ik_beam_select.restype = [_vp, ctypes.c_longlong, _vp, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp], _i
+        l.ik_copy_rows.argtypes, l.ik_copy_rows.restype = [_vp, _i, _vp, _i, _vp], _i
+        _search = l
+    return timed(_search)
+
+
+def _here(t: torch.Tensor, name: str) -> None:
+    if t.get_device() != torch.cuda.current_device():
+        raise KernelError(f"{name} is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+BEAMS_MOST, BEAM_OUT_MOST, BEAM_VOCAB_MOST = 16, 32, 1 << 20
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, n_out: int, out: Optional[torch.Tensor] = None):
+    """The best continuations of every request's beams.  ``logits`` [R * K, vocab] float32 (rows may have a stride), ``scores`` [R, K] float32:
+    each beam's sum of log probabilities so far (-inf: the beam is dead).  A candidate (beam, token) scores its beam's score plus the log
+    of its softmax probability.  Returns (scores [R, n_out] float32, beams [R, n_out] int32, tokens [R, n_out] int32) of the
+    best, descending, equal ones by ascending (beam, token); places without a candidate hold -inf, -1, -1.  Tokens whose logit is -inf or NaN are
+    no candidates.  ``out``: int32 [3, R, n_out] to write into (the scores' bits first); the results are views of it."""
+    _need(logits, "logits", torch.float32, contiguous=False)
+    _need(scores, "scores", torch.float32)
+    if logits.dim() != 2 or scores.dim() != 2 or scores.numel() != logits.shape[0]:
+        raise KernelError(f"beam_select: logits {tuple(logits.shape)} and scores {tuple(scores.shape)} do not go together ([R * K, vocab] and [R, K])")
+    (R, K), V = scores.shape, logits.shape[1]
+    if R == 0 or K == 0 or V == 0:
+        raise KernelError("beam_select: there is nothing to choose from")
+    if K > BEAMS_MOST or not 1 <= n_out <= BEAM_OUT_MOST or V > BEAM_VOCAB_MOST:
+        raise KernelError(f"beam_select: {K} beams, {n_out} results and a vocabulary of {V}: at most {BEAMS_MOST}, 1 to {BEAM_OUT_MOST} and {BEAM_VOCAB_MOST} are supported")
+    if logits.stride(1) != 1 and V > 1 or logits.stride(0) < V and R * K > 1:
+        raise KernelError("beam_select: the logits' rows must be contiguous and may not overlap")
+    _here(logits, "logits")
+    _here(scores, "scores")
+    if out is None:
+        out = torch.empty((3, R, n_out), dtype=torch.int32, device=logits.device)
+    else:
+        _need(out, "out", torch.int32)
+        _here(out, "out")
+        if out.shape != (3, R, n_out):
+            raise KernelError(f"beam_select: out must be [3, {R}, {n_out}], found {tuple(out.shape)}")
+    library = _search_lib()
+    need = library.ik_beam_select_scratch(R, K, V, n_out)
+    if need < 0:
+        raise KernelError("beam_select: these sizes are not supported")
+    scratch = torch.empty(need, dtype=torch.uint8, device=logits.device)
+    s, b, v = out.unbind(0)
+    _work(f"beam select {R}x{K}x{V}", R * K * V * 4 + need)
+    _check(library.ik_beam_select(_ptr(logits), logits.stride(0), _ptr(scores), R, K, V, n_out, _ptr(scratch), _ptr(s), _ptr(b), _ptr(v), _stream()),
+           "beam_select", kernels=2)
+    return s.view(torch.float32), b, v
+
+
+def copy_moves(src, dst, positions, rows: int, page: int) -> np.ndarray:
+    """The moves of one job of ``copy_rows`` as [n, 3] (source, destination, positions), checked."""
+    n = len(src)
+    if len(dst) != n or (positions is not None and len(positions) != n):
+        raise KernelError(f"copy_rows: {n} sources, {len(dst)} destinations" + ("" if positions is None else f", {len(positions)} numbers of positions"))
+    m = np.empty((n, 3), dtype=np.int64)
+    m[:, 0], m[:, 1], m[:, 2] = src, dst, 1 if positions is None else positions
+    if n and (m[:, :2].min() < 0 or m[:, :2].max() >= rows):
+        raise KernelError(f"copy_rows: a row is outside the tensor's {rows}")
+    if n and (m[:, 2].min() < 0 or m[:, 2].max() > page):
+        raise KernelError(f"copy_rows: a number of positions is outside [0, {page}]")
+    to = set(m[:, 1].tolist())
+    if len(to) != n or not to.isdisjoint(m[:, 0].tolist()):
+        raise KernelError("copy_rows: a row is written twice, or both read and written")
+    return m
+
+
+def copy_rows(jobs) -> None:
+    """Copies rows within tensors of a cache, all jobs in one launch.  A job is (tensor, src, dst, positions): ``tensor`` [entries, rows, ...] with everything behind
+    the first two dimensions contiguous; row src[i] is copied to row dst[i] in every entry.  ``positions``: None copies whole rows (states); else the
+    tensor is [entries, rows, heads, page, ...] and of every head the first positions[i] of a page are copied, what lies behind them in the destination stays.
+    src, dst and positions are host integers.  A row is not written twice, and none is both read and written: such a job is refused, and so are rows out of range
+    and jobs whose tensors overlap.  On refusal nothing has been copied."""
+    jobs = list(jobs)                              # the lists below are told apart by identity: they have to live until the end
+    table, moves, spans, nbytes = [], [], [], 0
+    n_moves = 0
+    seen = {}
+    for t, src, dst, positions in jobs:
+        if not t.is_cuda:
+            raise KernelError("copy_rows: a tensor must be a CUDA tensor (there is no CPU path)")
+        if t.dim() < 2 or (positions is not None and t.dim() < 4):
+            raise KernelError("copy_rows: a tensor is [entries, rows, ...], with positions [entries, rows, heads, page, ...]")
+        _here(t, "copy_rows: a tensor")
+        n = len(src)
+        if n == len(dst) == 0 or t.numel() == 0:
+            continue
+        shape, strides, size = t.shape, t.stride(), t.element_size()
+        inner = 1
+        for d in range(t.dim() - 1, 1, -1):
+            if shape[d] != 1 and strides[d] != inner:
+                raise KernelError("copy_rows: behind its first two dimensions a tensor must be contiguous")
+            inner *= shape[d]
+        fine = (shape[1] == 1 or strides[1] >= inner) and (shape[0] == 1 or strides[0] >= (shape[1] - 1) * strides[1] + inner
+                                                           or (strides[0] >= inner and strides[1] >= (shape[0] - 1) * strides[0] + inner))
+        if not fine or size % 2:
+            raise KernelError("copy_rows: a tensor's rows may not overlap, and an element has 2, 4, 8 or 16 bytes")
+        page = 1 if positions is None else shape[3]
+        key = (id(src), id(dst), id(positions), shape[1], page)
+        at = seen.get(key)
+        if at is None:
+            m = copy_moves(src, dst, positions, shape[1], page)
+            at = seen[key] = n_moves
+            moves.append(m)
+            n_moves += n
+        heads = 1 if positions is None else shape[2]
+        per_head = inner // heads * size
+        lo = t.data_ptr()
+        spans.append((lo, lo + ((shape[0] - 1) * strides[0] + (shape[1] - 1) * strides[1] + inner) * size))
+        table.append((lo, shape[0], strides[0] * size, shape[1], strides[1] * size, heads, per_head, per_head // page, at, n))
+        if _profile is not None:
+            nbytes += 2 * shape[0] * heads * (per_head // page) * int(moves[-1][:, 2].sum())
+    if not table:
+        return
+    spans.sort()
+    for a, b in zip(spans, spans[1:]):
+        if b[0] < a[1]:
+            raise KernelError("copy_rows: two jobs' tensors overlap")
+    j = np.array(table, dtype=np.int64)
+    m = (moves[0] if len(moves) == 1 else np.concatenate(moves)).astype(np.int32)
+    _work(f"copy rows {n_moves} moves in {len(table)} tensors", nbytes)
+    _check(_search_lib().ik_copy_rows(j.ctypes.data, len(table), m.ctypes.data, len(m), _stream()), "copy_rows")
 
 
 # ---------------------------------------------------------------------------------------------

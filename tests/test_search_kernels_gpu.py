@@ -1,0 +1,406 @@
+"""The kernels of a search over beams and of forked sequences against plain 64-bit forms: the choice of continuations, the copies of pages and
+states, attention behind shared pages."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+LOWEST = -3.4028234663852886e38
+
+
+def ops():
+    from ithaca_b200.csrc import ops as o
+    return o
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+# -- the choice of continuations -------------------------------------------------------------------------------------------
+def plain_scores(logits, sums):
+    """Scores [R, K * V] in 64 bits; -inf where there is no candidate."""
+    R, K = sums.shape
+    l = logits.double().view(R, K, -1)
+    l = torch.where(torch.isnan(l), -math.inf, l)
+    infinite = l == math.inf
+    share = infinite.any(-1, keepdim=True)
+    l = torch.where(share, torch.where(infinite, 0.0, -math.inf), l)
+    top = l.amax(-1, keepdim=True)
+    lse = torch.where(top > -math.inf, top + (l - torch.where(top > -math.inf, top, 0.0)).exp().sum(-1, keepdim=True).log(), 0.0)
+    c = sums.double()[..., None]
+    s = torch.where((c > -math.inf) & (l > -math.inf), c + (l - lse), -math.inf)
+    return s.flatten(1)
+
+
+# A float exponential is off by up to 2 units in the last place (2^-22), a thread adds 32 of them in float (32 x 2^-24), and the argument's
+# rounding is 2^-24 of it, weighted by the exponential: below 20 x 2^-24 on average.  All relative to the sum, so absolute in its logarithm.
+LSE = 2 ** -22 + 32 * 2 ** -24 + 20 * 2 ** -24
+
+
+def check_select(logits, sums, n):
+    got_s, got_b, got_v = (t.cpu() for t in ops().beam_select(logits.to(DEV), sums.to(DEV), n))
+    (R, K), V = sums.shape, logits.shape[1]
+    want = plain_scores(logits, sums)
+    assert got_s.shape == got_b.shape == got_v.shape == (R, n) and got_b.dtype == got_v.dtype == torch.int32
+    for r in range(R):
+        order = torch.sort(want[r], descending=True, stable=True)
+        best = [float(x) for x in order.values[:n] if x > -math.inf]
+        at = [int(b) * V + int(v) for b, v in zip(got_b[r], got_v[r])]
+        assert len(set(at[:len(best)])) == len(best)
+        for i in range(n):
+            if i >= len(best):
+                assert got_s[r, i] == -math.inf and got_b[r, i] == -1 and got_v[r, i] == -1
+                continue
+            assert 0 <= got_b[r, i] < K and 0 <= got_v[r, i] < V
+            # what was chosen at this rank is as good as the best there, to the errors of two sums
+            assert abs(float(want[r, at[i]]) - best[i]) <= 2 * LSE, (r, i, at[i], int(order.indices[i]))
+            assert abs(float(got_s[r, i]) - float(want[r, at[i]])) <= LSE + abs(best[i]) * 2 ** -24 + 1e-30
+            if i and got_b[r, i] == got_b[r, i - 1]:                        # within a beam the order is the logits' own
+                x, y = logits[r * K + got_b[r, i], got_v[r, i - 1]], logits[r * K + got_b[r, i], got_v[r, i]]
+                assert x > y or (x == y and got_v[r, i - 1] < got_v[r, i])
+    return got_s, got_b, got_v
+
+
+SIZES = [(1, 1, 1, 1), (1, 1, 5, 3), (1, 2, 3, 8), (2, 3, 17, 6), (3, 4, 1000, 8), (5, 5, 8192, 10), (1, 16, 8193, 32), (2, 2, 50257, 4), (1, 4, 128256, 8), (7, 1, 32000, 1),
+         (1, 16, 300001, 32), (33, 2, 256, 5)]
+
+
+@pytest.mark.parametrize("R,K,V,n", SIZES)
+def test_select_on_logits(R, K, V, n):
+    g = gen(V + n)
+    check_select(torch.randn((R * K, V), generator=g) * 3, torch.rand((R, K), generator=g) * -20, n)
+
+
+@pytest.mark.parametrize("kind", ["constant", "few values", "masked", "lowest", "one left", "none left", "nan", "infinite", "rising", "falling", "peaked"])
+@pytest.mark.parametrize("R,K,V,n", [(2, 3, 1001, 6), (1, 5, 20000, 32)])
+def test_select_on_rows_that_are_not_ordinary(kind, R, K, V, n):
+    g = gen(V)
+    l = torch.randn((R * K, V), generator=g) * 3
+    sums = torch.rand((R, K), generator=g) * -20
+    if kind == "constant":
+        l = torch.full_like(l, 0.25)
+    elif kind == "few values":
+        l = (l / 2).round() * 2
+    elif kind == "masked":
+        l[:, torch.rand(V, generator=g) < 0.995] = -math.inf
+    elif kind == "lowest":
+        l[:, torch.rand(V, generator=g) < 0.999] = LOWEST
+    elif kind in ("one left", "none left"):
+        l[0] = -math.inf
+        l[1] = -math.inf
+        if kind == "one left":
+            l[1, V - 1] = -5.0
+    elif kind == "nan":
+        l[torch.rand((R * K, V), generator=g) < 0.01] = math.nan
+        l[1] = math.nan
+    elif kind == "infinite":
+        l[0, 7] = l[0, 500] = l[1, V - 1] = math.inf
+    elif kind == "rising":
+        l = l.sort(1).values
+    elif kind == "falling":
+        l = l.sort(1, descending=True).values
+    else:
+        l[:, 321] += 60.0
+    check_select(l, sums, n)
+
+
+def test_equal_candidates_come_by_beam_and_token():
+    """Equal beams (odd vocabularies: their rows start on different alignments) with equal sums: every rank has an exact tie."""
+    for V, n in ((1001, 8), (20003, 32), (128256, 16)):
+        row = torch.randn((1, V), generator=gen(V)).repeat(4, 1)
+        s, b, v = ops().beam_select(row.to(DEV), torch.full((1, 4), -3.0, device=DEV), n)
+        top = torch.sort(row[0], descending=True, stable=True).indices
+        assert b[0].tolist() == [i % 4 for i in range(n)]
+        assert v[0].tolist() == [int(top[i // 4]) for i in range(n)]
+    flat = torch.zeros((3, 70000), device=DEV)
+    s, b, v = ops().beam_select(flat, torch.zeros((1, 3), device=DEV), 20)
+    assert b[0].tolist() == [0] * 20 and v[0].tolist() == list(range(20))
+
+
+def test_dead_beams_are_left_alone():
+    g = gen(3)
+    l = torch.randn((8, 501), generator=g)
+    sums = torch.tensor([[-math.inf, -2.0, -math.inf, -1.0], [-math.inf] * 4])
+    sums[0, 2] = math.nan
+    l[0], l[2] = math.nan, math.inf
+    check = torch.where(torch.isnan(sums), -math.inf, sums)
+    s, b, v = ops().beam_select(l.to(DEV), sums.to(DEV), 8)
+    assert set(b[0].tolist()) <= {1, 3} and b[1].tolist() == [-1] * 8 and v[1].tolist() == [-1] * 8
+    check_select(torch.where(torch.isnan(l) | (l == math.inf), 0.0, l), check, 8)
+
+
+def test_select_reads_rows_with_a_stride_and_writes_where_it_is_told():
+    g = gen(5)
+    wide = torch.randn((6, 900), generator=g)
+    sums = torch.rand((2, 3), generator=g) * -4
+    for lo, hi in ((0, 800), (1, 800), (3, 64), (7, 900)):
+        view = wide.to(DEV)[:, lo:hi]
+        assert not view.is_contiguous()
+        out = torch.full((3, 2, 6), 77, dtype=torch.int32, device=DEV)
+        got = ops().beam_select(view, sums.to(DEV), 6, out=out)
+        want = ops().beam_select(wide[:, lo:hi].contiguous().to(DEV), sums.to(DEV), 6)
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+        assert torch.equal(out[1], want[1]) and torch.equal(out[0].view(torch.float32), want[0])
+
+
+def test_select_on_another_stream_and_replayed():
+    g = gen(6)
+    l, sums = (torch.randn((8, 33000), generator=g)).to(DEV), (torch.rand((2, 4), generator=g) * -9).to(DEV)
+    want = [t.clone() for t in ops().beam_select(l, sums, 8)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = [t.clone() for t in ops().beam_select(l, sums, 8)]
+    torch.cuda.synchronize()
+    graph, out = torch.cuda.CUDAGraph(), torch.zeros((3, 2, 8), dtype=torch.int32, device=DEV)
+    with torch.cuda.graph(graph):
+        ops().beam_select(l, sums, 8, out=out)
+    for shift in (0, 1):
+        rolled = l.roll(shift * 4, 0).clone()
+        other = [t.clone() for t in ops().beam_select(rolled, sums, 8)]
+        l.copy_(rolled)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out[0].view(torch.float32), other[0]) and torch.equal(out[1], other[1]) and torch.equal(out[2], other[2])
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_select_refuses():
+    o = ops()
+    l, s = torch.zeros((4, 10), device=DEV), torch.zeros((2, 2), device=DEV)
+    for bad in (lambda: o.beam_select(l.double(), s, 2), lambda: o.beam_select(l, s.half(), 2), lambda: o.beam_select(l.cpu(), s, 2), lambda: o.beam_select(l, s.cpu(), 2),
+                lambda: o.beam_select(l, s, 0), lambda: o.beam_select(l, s, 33), lambda: o.beam_select(l[:3], s, 2), lambda: o.beam_select(l.t(), s, 2),
+                lambda: o.beam_select(torch.zeros((17, 10), device=DEV), torch.zeros((1, 17), device=DEV), 2), lambda: o.beam_select(l[:, :0], s, 2),
+                lambda: o.beam_select(l[:0], s[:0], 2), lambda: o.beam_select(l, s, 2, out=torch.zeros((3, 2, 3), dtype=torch.int32, device=DEV)),
+                lambda: o.beam_select(l[:1].expand(4, 10), s, 2)):
+        with pytest.raises(o.KernelError):
+            bad()
+
+
+# -- copies ----------------------------------------------------------------------------------------------------------------
+def plain_copy(t, src, dst, positions):
+    t = t.clone()
+    old = t.clone()
+    for i, (s, d) in enumerate(zip(src, dst)):
+        if positions is None:
+            t[:, d] = old[:, s]
+        else:
+            t[:, d, :, :positions[i]] = old[:, s, :, :positions[i]]
+    return t
+
+
+@pytest.mark.parametrize("shape,dtype,whole", [((2, 9, 3, 64, 16), torch.bfloat16, False), ((3, 9, 2, 64, 33), torch.bfloat16, False), ((1, 9, 1, 64, 5), torch.float32, False),
+                                               ((5, 9, 4, 64), torch.float32, False), ((2, 9, 8, 64, 128), torch.bfloat16, False), ((3, 9, 7), torch.float32, True),
+                                               ((2, 9, 2, 4099), torch.float32, True), ((2, 9, 3), torch.bfloat16, True), ((4, 9, 2, 16, 64, 64), torch.float32, True),
+                                               ((2, 9, 5), torch.int32, True)])
+def test_copies_of_pages_and_states(shape, dtype, whole):
+    g = gen(sum(shape))
+    t = (torch.randn(shape, generator=g) * 100).to(dtype)
+    src, dst = [4, 4, 4, 0, 7, 7], [1, 8, 2, 3, 5, 6]
+    for positions in ([None] if whole else [[64] * 6, [1] * 6, [0, 5, 5, 63, 64, 17]]):
+        d = t.to(DEV)
+        ops().copy_rows([(d, src, dst, positions)])
+        assert torch.equal(d.cpu(), plain_copy(t, src, dst, positions))
+
+
+def test_copies_in_several_tensors_and_long_lists():
+    """Lists beyond what one launch carries, several tensors with lists of their own, a fan of destinations wider than a move carries."""
+    g = gen(1)
+    k, v = torch.randn((2, 500, 2, 64, 16), generator=g).to(torch.bfloat16), torch.randn((2, 500, 2, 64, 24), generator=g).to(torch.bfloat16)
+    st = [torch.randn((3, 40, 11), generator=g) for _ in range(20)]
+    order = torch.randperm(500, generator=g).tolist()
+    src, dst = [order[0]] * 30 + order[1:220], order[220:469]
+    rows = torch.randint(0, 65, (249,), generator=g).tolist()
+    slots = torch.randperm(40, generator=g).tolist()
+    gpu = [t.to(DEV) for t in (k, v, *st)]
+    ops().copy_rows([(gpu[0], src, dst, rows), (gpu[1], src, dst, rows)] + [(t, slots[:i], slots[20:20 + i], None) for i, t in enumerate(gpu[2:])])
+    want = [plain_copy(k, src, dst, rows), plain_copy(v, src, dst, rows)] + [plain_copy(t, slots[:i], slots[20:20 + i], None) for i, t in enumerate(st)]
+    for a, b in zip(gpu, want):
+        assert torch.equal(a.cpu(), b)
+    ops().copy_rows([])
+    ops().copy_rows([(gpu[0], [], [], [])])
+    assert torch.equal(gpu[0].cpu(), want[0])
+
+
+def test_copies_within_views():
+    """A layer's own part of a cache, rows with a stride, one entry of many."""
+    base = torch.randn((4, 10, 2, 64, 8), generator=gen(2))
+    d = base.to(DEV)
+    ops().copy_rows([(d[1:2], [3], [5], [9]), (d[2:, 1::2], [0, 0], [1, 4], [64, 64])])
+    want = base.clone()
+    want[1:2] = plain_copy(base[1:2], [3], [5], [9])
+    want[2:, 1::2] = plain_copy(base[2:, 1::2], [0, 0], [1, 4], [64, 64])
+    assert torch.equal(d.cpu(), want)
+
+
+def test_a_captured_copy_keeps_its_lists():
+    d = torch.arange(60, dtype=torch.float32, device=DEV).view(1, 20, 3).clone()
+    ops().copy_rows([(d, [0], [1], None)])
+    graph, src, dst = torch.cuda.CUDAGraph(), [2, 2], [3, 4]
+    with torch.cuda.graph(graph):
+        ops().copy_rows([(d, src, dst, None)])
+    src[:], dst[:] = [9, 9], [0, 1]
+    d[0, 2] = 5.0
+    graph.replay()
+    torch.cuda.synchronize()
+    assert d[0, 3].tolist() == d[0, 4].tolist() == [5.0] * 3 and d[0, 0].tolist() == [0.0, 1.0, 2.0]
+
+
+def test_copies_are_refused_whole():
+    o = ops()
+    t = torch.arange(2 * 6 * 2 * 64 * 4, dtype=torch.float32, device=DEV).view(2, 6, 2, 64, 4)
+    keep = t.clone()
+    for bad in ([(t, [0], [6], None)], [(t, [-1], [2], None)], [(t, [0, 1], [2, 2], None)], [(t, [0, 1], [1, 2], None)], [(t, [0], [0], None)], [(t, [0], [1], [65])],
+                [(t, [0], [1], [-1])], [(t, [0, 1], [2], None)], [(t, [0], [1], [])], [(t.cpu(), [0], [1], None)], [(t.transpose(3, 4), [0], [1], None)],
+                [(t[0, 0, 0], [0], [1], [3])], [(t, [1], [2], None), (t, [3], [4], None)], [(t, [1], [2], None), (t[1:], [3], [4], None)],
+                [(t, [1], [2], None), (torch.zeros((1, 3), dtype=torch.int8, device=DEV), [0], [1], None)]):
+        with pytest.raises(o.KernelError):
+            o.copy_rows(bad)
+    assert torch.equal(t, keep)
+
+
+# -- attention behind shared pages -----------------------------------------------------------------------------------------
+def layout(members, shared, lens, seed, extra=3):
+    """A block table in which every group's members name the same first pages, all pages in random order."""
+    owns = [-(-n // 64) for n in lens]
+    total = sum(shared) + sum(owns) + extra
+    order = torch.randperm(total, generator=gen(seed)).tolist()
+    table, b = torch.full((len(lens), max(1, max(owns))), -1, dtype=torch.int32), 0
+    for m, s in zip(members, shared):
+        first, order = order[:s], order[s:]
+        for _ in range(m):
+            rest, order = order[:max(0, owns[b] - s)], order[max(0, owns[b] - s):]
+            table[b, :owns[b]] = torch.tensor((first + rest)[:owns[b]], dtype=torch.int32)
+            b += 1
+    return table, total
+
+
+def run_shared(nh, nkv, hd, members, shared, lens, seed=0, softcap=0.0, sink=False, chunks=None, scale=None, garbage=True, bounds=None):
+    from ithaca_b200.csrc import attention_bf16
+    g = gen(seed + hd)
+    table, total = layout(members, shared, lens, seed)
+    B, scale = len(lens), scale or hd ** -0.5
+    q = torch.randn((B, nh * hd), generator=g).to(torch.bfloat16)
+    k, v = ((torch.randn((total, nkv, 64, hd), generator=g) * f).to(torch.bfloat16) for f in (1.5, 1.0))
+    if garbage:                                                     # behind a sequence's last key anything may lie
+        for b, n in enumerate(lens):
+            if n % 64:
+                k[table[b, n // 64], :, n % 64:] = math.nan
+                v[table[b, n // 64], :, n % 64:] = math.inf
+    per = [s for m, s in zip(members, shared) for _ in range(m)]
+    starts = torch.tensor([0] + torch.tensor(members).cumsum(0).tolist(), dtype=torch.int32)
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    owns = [-(-n // 64) - s for n, s in zip(lens, per)]
+    got = attention_bf16.decode_shared(q.to(DEV), k.to(DEV), v.to(DEV), torch.tensor(lens, dtype=torch.int32, device=DEV), table.to(DEV), starts.to(DEV),
+                                       torch.tensor(per, dtype=torch.int32, device=DEV), len(members), max(members), *(bounds or (max(shared), max(owns))), nh, scale, status,
+                                       softcap=softcap, sink=sink.to(DEV) if torch.is_tensor(sink) else sink, chunks=chunks).cpu().double().view(B, nh, hd)
+    assert status.item() == 0
+    for b, n in enumerate(lens):
+        if n == 0:
+            assert (got[b] == 0).all()
+            continue
+        pages = table[b, :-(-n // 64)].long()
+        kb, vb = (t[pages].double().transpose(0, 1).reshape(nkv, -1, hd)[:, :n].repeat_interleave(nh // nkv, 0) for t in (k, v))
+        s = torch.einsum("hd,hjd->hj", q[b].double().view(nh, hd), kb) * scale
+        if softcap:
+            s = softcap * torch.tanh(s / softcap)
+        top = s.amax(-1, keepdim=True)
+        sinks = sink.double()[:, None] if torch.is_tensor(sink) else torch.zeros((nh, 1), dtype=torch.float64)
+        if torch.is_tensor(sink) or sink:
+            top = torch.maximum(top, sinks)
+        p = (s - top).exp()
+        total_p = p.sum(-1, keepdim=True) + ((sinks - top).exp() if torch.is_tensor(sink) or sink else 0.0)
+        want = torch.einsum("hj,hjd->hd", p, vb) / total_p
+        size = torch.einsum("hj,hjd->hd", p, vb.abs()) / total_p
+        # a probability and the result are rounded to bfloat16 (2^-8 each); a score is a float sum of hd products (about hd 2^-24 of their sizes, below
+        # 2^-14 here), which the exponential passes on; the cap's tanh is off by up to 2^-11 of the cap
+        tol = 2 ** -8 * (size + want.abs()) + 2 ** -14 * size + (softcap * 2 ** -10 * size if softcap else 0.0)
+        assert torch.isfinite(got[b]).all()
+        assert ((got[b] - want).abs() <= tol).all(), (b, ((got[b] - want).abs() / tol).max())
+
+
+@pytest.mark.parametrize("nh,nkv,hd", [(32, 8, 128), (32, 8, 64), (8, 8, 16), (6, 2, 48), (40, 40, 128), (20, 1, 64), (6, 3, 80), (4, 2, 256), (64, 8, 128)])
+@pytest.mark.parametrize("members,shared,lens", [
+    ([4], [2], [129, 129, 129, 129]),                               # a tail of one key
+    ([1], [0], [1]),                                                 # one sequence, one key
+    ([3, 1, 2], [5, 0, 1], [321, 330, 450, 70, 65, 128]),            # unequal groups, one alone, a tail that fills its page
+    ([2, 2], [0, 3], [5, 64, 200, 256]),                             # a group that shares nothing yet
+    ([16], [1], [65 + 3 * i for i in range(16)]),
+    ([2, 3], [1, 0], [64, 100, 0, 1, 63]),                           # nothing behind the shared page; a sequence without keys
+])
+def test_attention_behind_shared_pages(nh, nkv, hd, members, shared, lens):
+    run_shared(nh, nkv, hd, members, shared, lens, seed=len(lens))
+
+
+@pytest.mark.parametrize("chunks", [(1, 1), (2, 1), (3, 5), (64, 64)])
+def test_every_cut_of_the_pages(chunks):
+    run_shared(8, 2, 64, [3, 2], [7, 4], [449, 500, 700, 257, 300], seed=4, chunks=chunks)
+    run_shared(8, 2, 128, [3, 2], [7, 4], [449, 500, 700, 257, 300], seed=5, chunks=chunks)
+
+
+def test_bounds_that_are_too_small_cost_time_only():
+    for bounds in ((1, 1), (0, 0), (3, 2), (100, 100)):
+        run_shared(8, 2, 64, [3, 2], [7, 4], [449, 500, 700, 257, 300], seed=4, bounds=bounds)
+
+
+def test_cap_sink_and_scale():
+    run_shared(8, 2, 64, [3, 2], [3, 4], [200, 211, 340, 257, 300], seed=6, softcap=20.0, scale=0.3)
+    run_shared(8, 2, 64, [3, 2], [3, 4], [200, 211, 340, 257, 300], seed=7, sink=True)
+    run_shared(8, 2, 64, [3, 2], [3, 4], [200, 211, 340, 257, 0], seed=8, sink=torch.randn(8, generator=gen(9)) * 3)
+
+
+def test_a_group_of_everything_and_long_prompts():
+    run_shared(32, 8, 128, [8, 8], [130, 33], [130 * 64 + 70 + i for i in range(8)] + [33 * 64 + 1] * 8, seed=10)
+
+
+def test_pages_outside_the_pool_are_not_followed():
+    from ithaca_b200.csrc import attention_bf16
+    k = torch.randn((6, 2, 64, 64), device=DEV).to(torch.bfloat16)
+    q = torch.randn((4, 256), device=DEV).to(torch.bfloat16)
+    args = (torch.tensor([130] * 4, dtype=torch.int32, device=DEV),)
+    for table in ([[0, 99, 1]] * 4, [[0, 1, -1]] * 4):
+        status = torch.zeros(1, dtype=torch.int32, device=DEV)
+        attention_bf16.decode_shared(q, k, k, *args, torch.tensor(table, dtype=torch.int32, device=DEV), torch.tensor([0, 4], dtype=torch.int32, device=DEV),
+                                     torch.tensor([2] * 4, dtype=torch.int32, device=DEV), 1, 4, 2, 1, 4, 0.125, status)
+        assert status.item() == 1 << 2
+
+
+def test_shared_attention_replayed_for_other_lengths():
+    from ithaca_b200.csrc import attention_bf16
+    g = gen(11)
+    k, v = (torch.randn((40, 2, 64, 64), generator=g).to(torch.bfloat16).to(DEV) for _ in range(2))
+    q = torch.randn((4, 512), generator=g).to(torch.bfloat16).to(DEV)
+    table = torch.stack([torch.cat((torch.arange(6), 6 + 6 * i + torch.arange(6))) for i in range(4)]).to(torch.int32).to(DEV)
+    lens, starts, shared = (torch.tensor(x, dtype=torch.int32, device=DEV) for x in ([400] * 4, [0, 2, 4], [6] * 4))
+    status, out = torch.zeros(1, dtype=torch.int32, device=DEV), torch.empty_like(q)
+    call = lambda o=None: attention_bf16.decode_shared(q, k, v, lens, table, starts, shared, 2, 2, 6, 6, 8, 0.125, status, out=o)
+    call(out)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(out)
+    for n, s in (([400, 401, 600, 768], [6] * 4), ([700, 390, 450, 500], [3, 3, 6, 6]), ([1, 2, 3, 4], [0] * 4)):
+        lens.copy_(torch.tensor(n, dtype=torch.int32))
+        shared.copy_(torch.tensor(s, dtype=torch.int32))
+        graph.replay()
+        assert torch.equal(out, call())
+    assert status.item() == 0
+
+
+def test_shared_attention_refuses():
+    from ithaca_b200.csrc import attention_bf16
+    o = ops()
+    k = torch.zeros((6, 2, 64, 64), dtype=torch.bfloat16, device=DEV)
+    q = torch.zeros((4, 256), dtype=torch.bfloat16, device=DEV)
+    ints = lambda *x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    good = dict(q=q, k_pages=k, v_pages=k, kv_lens=ints(70, 70, 70, 70), table=torch.zeros((4, 2), dtype=torch.int32, device=DEV), starts=ints(0, 4), shared=ints(1, 1, 1, 1),
+                n_groups=1, max_members=4, shared_bound=1, own_bound=1, n_heads=4, scale=0.125, status=None)
+    attention_bf16.decode_shared(**good)
+    for bad in (dict(q=q.float()), dict(k_pages=k.float()), dict(v_pages=k[:5]), dict(n_heads=3), dict(q=q[:3]), dict(starts=ints(0, 2, 4)), dict(shared=ints(1, 1)), dict(max_members=0),
+                dict(max_members=5), dict(table=good["table"][:3]), dict(table=good["table"].long()), dict(kv_lens=good["kv_lens"].cpu()), dict(k_pages=k[:, :, :32], v_pages=k[:, :, :32]),
+                dict(sink=torch.zeros(3, device=DEV)), dict(k_pages=k[..., :24], v_pages=k[..., :24])):
+        with pytest.raises(o.KernelError):
+            attention_bf16.decode_shared(**{**good, **bad})
