@@ -7,10 +7,10 @@ generation loop with sampling, and hand-written CUDA kernels for sm_100a beside 
 true 32-bit path.
 """
 from .config import LlamaConfig, register_architecture, registered_architectures
-from .engine import Engine, GenerationOptions, GenStats
+from .engine import BeamOptions, Engine, GenerationOptions, GenStats, Hypothesis
 from .sampling import SamplingOptions
 from .weights import write_random_model
 
-__all__ = ["Engine", "GenerationOptions", "GenStats", "SamplingOptions", "LlamaConfig", "register_architecture",
+__all__ = ["BeamOptions", "Engine", "GenerationOptions", "GenStats", "Hypothesis", "SamplingOptions", "LlamaConfig", "register_architecture",
            "registered_architectures", "write_random_model"]
 __version__ = "0.1.0"

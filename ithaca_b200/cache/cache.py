@@ -156,6 +156,29 @@ class SequenceCache:
     def free_slot(self, slot: int) -> None:
         self.table.free_slot(slot)
 
+    def fork(self, wanted: Sequence[Tuple[int, int]]) -> List[List[int]]:
+        """For every (slot, n): n new slots that hold what the slot holds.  Full pages are shared; pages that are only begun and fixed-size
+        states are copied, all layers and slots in one launch.  CacheFull if slots or pages do not suffice; nothing has changed then."""
+        made, copies = self.table.fork(wanted)
+        src = [slot for (slot, _), new in zip(wanted, made) for _ in new]
+        self._copy(copies, src, [s for new in made for s in new])
+        return made
+
+    def _copy(self, pages: Sequence[Sequence[Tuple[int, int, int]]], from_slots: Sequence[int], to_slots: Sequence[int]) -> None:
+        """Copies of begun pages (per key/value group: source, destination, filled positions) and of slots' states."""
+        if self.device is None:
+            return
+        jobs = []
+        for g, moves in enumerate(pages):
+            if moves:
+                src, dst, rows = zip(*moves)
+                jobs += [(t, src, dst, rows) for t in (self.k[g], self.v[g], self.key_scales[g]) if t is not None and t.numel()]
+        if to_slots:
+            jobs += [(t, from_slots, to_slots, None) for t in self.state]
+        if jobs:
+            from ..csrc import ops
+            ops.copy_rows(jobs)
+
     def length(self, slot: int) -> int:
         self.table._check_slot(slot)
         return int(self.table.length[slot])
@@ -167,7 +190,7 @@ class SequenceCache:
         if self.state_groups and n not in (0, self.length(slot)):
             raise CacheError("a sequence with fixed-size state can only be truncated to 0")
         shorter = n < self.length(slot)
-        self.table.truncate(slot, n)
+        self._copy(self.table.truncate(slot, n), [], [])
         if n == 0 and shorter:
             for t in self.state:
                 t[:, slot].zero_()

@@ -9,11 +9,15 @@ pools of their own: a group that keeps every key never releases a page before
 the slot is freed; a group with a window releases pages that no later query can
 reach (those of a sequence's first ``keep_first`` keys stay).  Slots and pages go back to their pools when a sequence ends and are
 handed out again.
+
+A slot can be forked: the new slot holds the same positions.  Full pages are then held by both (a pool counts a page's
+holders; it is free again when the last one has given it back), and a page that is only begun is copied, so that a page
+with several holders is never written: what the tables name twice is full.
 """
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Dict, List, Optional, Sequence
+from typing import List, Optional, Sequence, Tuple
 
 import numpy as np
 
@@ -27,14 +31,15 @@ class CacheFull(CacheError):
 
 
 class PagePool:
-    """A fixed set of page ids.  A page is either free or held by exactly one owner."""
+    """A fixed set of page ids.  A page is either free or held, by one owner or by several that share it."""
 
     def __init__(self, n_pages: int):
         if n_pages < 0:
             raise CacheError(f"a pool cannot have {n_pages} pages")
         self.n_pages = n_pages
         self._free: List[int] = list(range(n_pages - 1, -1, -1))   # pop() hands out low ids first
-        self._held = np.zeros(n_pages, dtype=bool)
+        self._holders = np.zeros(n_pages, dtype=np.int32)
+        self.n_shared = 0                                          # pages with more than one holder
 
     @property
     def n_free(self) -> int:
@@ -44,21 +49,40 @@ class PagePool:
         if not self._free:
             raise CacheFull(f"the cache is full: all {self.n_pages} pages are in use")
         p = self._free.pop()
-        if self._held[p]:
+        if self._holders[p]:
             raise CacheError(f"page {p} was on the free list while held")
-        self._held[p] = True
+        self._holders[p] = 1
         return p
 
-    def give_back(self, page: int) -> None:
+    def _check(self, page: int) -> None:
         if not 0 <= page < self.n_pages:
             raise CacheError(f"page {page} does not belong to this pool of {self.n_pages}")
-        if not self._held[page]:
+
+    def share(self, page: int) -> None:
+        """One more holder for a held page."""
+        self._check(page)
+        if not self._holders[page]:
+            raise CacheError(f"page {page} is free and cannot be shared")
+        self._holders[page] += 1
+        self.n_shared += self._holders[page] == 2
+
+    def holders(self, page: int) -> int:
+        self._check(page)
+        return int(self._holders[page])
+
+    def give_back(self, page: int) -> None:
+        """One holder less; the page is free when none is left."""
+        self._check(page)
+        if not self._holders[page]:
             raise CacheError(f"page {page} is freed twice")
-        self._held[page] = False
-        self._free.append(page)
+        self._holders[page] -= 1
+        if self._holders[page] == 0:
+            self._free.append(page)
+        elif self._holders[page] == 1:
+            self.n_shared -= 1
 
     def held(self) -> int:
-        return int(self._held.sum())
+        return int((self._holders > 0).sum())
 
 
 @dataclass(frozen=True)
@@ -130,6 +154,44 @@ class SlotTable:
         self.length[slot] = 0
         self._reserved[slot] = 0
         self._free_slots.append(slot)
+
+    def fork(self, wanted: Sequence[Tuple[int, int]]):
+        """For every (slot, n): n new slots that hold the same positions.  Full pages are shared; where the last page is only begun
+        every new slot gets one of its own.  Returns (the new slots per entry, per group the copies that make those pages what
+        they stand for: (source page, destination page, filled positions)).  On refusal nothing has changed."""
+        for slot, n in wanted:
+            self._check_slot(slot)
+            if n < 0:
+                raise CacheError("cannot fork a slot a negative number of times")
+        total = sum(n for _, n in wanted)
+        if total > len(self._free_slots):
+            raise CacheFull(f"{total} more slots are needed, {len(self._free_slots)} of {self.max_slots} are free")
+        begun = sum(n for slot, n in wanted if self.length[slot] % self.page_size)
+        for g, pool in enumerate(self.pools):
+            if pool.n_free < begun:
+                raise CacheFull(f"the cache is full: {begun} more pages of {self.page_size} positions are needed in group {g}, {pool.n_free} of {pool.n_pages} are free")
+        made: List[List[int]] = []
+        copies: List[List[Tuple[int, int, int]]] = [[] for _ in self.pools]
+        for slot, n in wanted:
+            length = int(self.length[slot])
+            full, rows = divmod(length, self.page_size)
+            made.append([])
+            for _ in range(n):
+                new = self.alloc_slot()
+                for g, pool in enumerate(self.pools):
+                    mine, row = self.tables[g][slot], self.tables[g][new]
+                    row[:full] = mine[:full]
+                    for p in mine[:full]:
+                        if p >= 0:
+                            pool.share(int(p))
+                    if rows:
+                        row[full] = pool.take()
+                        copies[g].append((int(mine[full]), int(row[full]), rows))
+                    self._first_live[g][new] = self._first_live[g][slot]
+                self.length[new] = length
+                self._reserved[new] = -(-length // self.page_size) * self.page_size
+                made[-1].append(new)
+        return made, copies
 
     def in_use(self, slot: int) -> bool:
         return 0 <= slot < self.max_slots and bool(self._in_use[slot])
@@ -205,11 +267,13 @@ class SlotTable:
         """Table columns that a windowed group never releases: the pages of its kept first keys."""
         return -(-grp.keep_first // self.page_size)
 
-    def truncate(self, slot: int, n: int) -> None:
+    def truncate(self, slot: int, n: int) -> List[List[Tuple[int, int, int]]]:
         """Keeps the first ``n`` positions (the reference's ``rewind``, src/model.cpp:1047-1058).
-        Pages past them are kept for reuse by the same slot.  A windowed group cannot go
+        Pages past them are kept for reuse by the same slot, unless some of them are shared: those are not this slot's to write, and all
+        past the cut are given back.  A windowed group cannot go
         back behind pages it has already released, except to 0: then the slot gives all its
-        pages back and starts again.  On refusal nothing has changed."""
+        pages back and starts again.  Returns per group the copies that ``fork`` returns: where the cut lies inside a shared page the slot gets one of its own.
+        On refusal nothing has changed."""
         self._check_slot(slot)
         if not 0 <= n <= self.length[slot]:
             raise CacheError(f"slot {slot}: cannot truncate to {n}, it holds {int(self.length[slot])}")
@@ -222,14 +286,37 @@ class SlotTable:
                 self._first_live[g][slot] = 0
             self.length[slot] = 0
             self._reserved[slot] = 0
-            return
+            return [[] for _ in self.pools]
         for g, grp in enumerate(self.kv_groups):
             if grp.window is not None and n < self.length[slot]:
                 first_needed = max(0, n + 1 - grp.window)
                 # the released columns are those between the kept ones and the first live one
                 if max(first_needed // self.page_size, self._kept_cols(grp)) < self._first_live[g][slot]:
                     raise CacheError(f"slot {slot}: group {g} has released the pages a truncation to {n} would need")
+        copies: List[List[Tuple[int, int, int]]] = [[] for _ in self.pools]
+        if any(pool.n_shared for pool in self.pools):
+            begun, rows = divmod(n, self.page_size)
+            keep = begun + (rows > 0)
+            past = [[int(p) for p in self.tables[g][slot][keep:] if p >= 0] for g in range(len(self.pools))]
+            drop = any(pool.holders(p) > 1 for pool, pages in zip(self.pools, past) for p in pages)
+            own = [bool(rows) and self.tables[g][slot][begun] >= 0 and pool.holders(int(self.tables[g][slot][begun])) > 1 for g, pool in enumerate(self.pools)]
+            for g, pool in enumerate(self.pools):
+                if own[g] and pool.n_free == 0 and not (drop and any(pool.holders(p) == 1 for p in past[g])):
+                    raise CacheFull(f"the cache is full: slot {slot} needs a page of its own in group {g} to be cut to {n}, all {pool.n_pages} are in use")
+            for g, pool in enumerate(self.pools):
+                row = self.tables[g][slot]
+                if drop:
+                    for p in past[g]:
+                        pool.give_back(p)
+                    row[keep:] = -1
+                if own[g]:
+                    old, row[begun] = int(row[begun]), pool.take()
+                    pool.give_back(old)
+                    copies[g].append((old, int(row[begun]), rows))
+            if drop:
+                self._reserved[slot] = keep * self.page_size
         self.length[slot] = n
+        return copies
 
     def table_rows(self, group: int, slots: Sequence[int], n_cols: int) -> np.ndarray:
         """[len(slots), n_cols] block table of the given slots (padded with -1)."""
@@ -240,15 +327,22 @@ class SlotTable:
         return out
 
     def check_consistent(self) -> None:
-        """Every page is free or held by exactly one table entry (used by the tests)."""
+        """Every page is free or held by as many table entries as its pool counts, and a page that several hold is full in all of
+        them (used by the tests)."""
         for g, pool in enumerate(self.pools):
             t = self.tables[g]
-            used = t[t >= 0]
-            if len(np.unique(used)) != len(used):
+            used, times = np.unique(t[t >= 0], return_counts=True)
+            if np.any(pool._holders[used] < times):
                 raise CacheError(f"group {g}: a page is held twice")
             if len(used) != pool.held():
                 raise CacheError(f"group {g}: {pool.held()} pages are held but the tables name {len(used)}")
+            if np.any(pool._holders[used] != times) or pool.n_shared != int((times > 1).sum()):
+                raise CacheError(f"group {g}: a page's holders are not those that the tables name")
             if len(used) + pool.n_free != pool.n_pages:
                 raise CacheError(f"group {g}: pages were lost ({len(used)} held + {pool.n_free} free != {pool.n_pages})")
             if np.any(t[~self._in_use] >= 0):
                 raise CacheError(f"group {g}: a free slot still holds pages")
+            for p in used[times > 1]:
+                slots, cols = np.nonzero(t == p)
+                if np.any((cols + 1) * self.page_size > self.length[slots]):
+                    raise CacheError(f"group {g}: page {int(p)} is shared but not full")

@@ -245,6 +245,11 @@ def shared_chunks(n_groups: int, max_members: int, n_seqs: int, n_heads: int, n_
     return max(2, -(-max(1, shared_bound) // n_shared)), 4
 
 
+def sharing_pays(starts, pages, n_pages, n_kv_heads: int, hd: int) -> bool:
+    """Whether a decode step whose sequences share pages so reads them once per group."""
+    return True
+
+
 def decode_shared(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, kv_lens: torch.Tensor, table: torch.Tensor, starts: torch.Tensor,
                   shared: torch.Tensor, n_groups: int, max_members: int, shared_bound: int, own_bound: int, n_heads: int, scale: float,
                   status: Optional[torch.Tensor], out: Optional[torch.Tensor] = None, softcap: float = 0.0, sink=False,
@@ -288,9 +293,9 @@ def decode_shared(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
 
 def attend(q, k_pages, v_pages, ctx, table, n_heads: int, scale: float, window: int,
            status, softcap: float = 0.0, sink=False, keep: int = 0,
-            key_scales: Optional[torch.Tensor] = None, slopes: Optional[torch.Tensor] = None, reach=None) -> Optional[torch.Tensor]:
+            key_scales: Optional[torch.Tensor] = None, slopes: Optional[torch.Tensor] = None, reach=None, sharing=None) -> Optional[torch.Tensor]:
     """Returns None when no specialised kernel takes these sizes or options (the caller then uses the
-    CUDA-core kernel)."""
+    CUDA-core kernel).  ``sharing``: which neighbours of a decode step share their first pages (``engine.context.Sharing``), or None."""
     n_pages, nkv, page_size, hd = k_pages.shape
     if k_pages.dtype != torch.bfloat16 or q.dtype != torch.bfloat16 or page_size != 64 or not supported(hd):
         return None
@@ -304,6 +309,12 @@ def attend(q, k_pages, v_pages, ctx, table, n_heads: int, scale: float, window: 
         keys = sum(min(e, window + keep + n) if window else e for n, e in zip(ctx.host_n_new, ctx.host_kv_lens))
         rows = hd * 2 + 4 if key_scales is not None else 2 * hd * 2             # bytes of a key (and value) per kv head
         work = (2 * q.numel() * 2 + keys * nkv * rows, 4 * hd * n_heads * pairs)
+    if ctx.is_decode and sharing is not None and not window and key_scales is None and slopes is None:
+        if work is not None:
+            once = sum((b - a - 1) * sharing.pages[a] * page_size for a, b in zip(sharing.starts, sharing.starts[1:]))
+            work = (work[0] - once * nkv * 4 * hd, work[1])
+        return decode_shared(q, k_pages, v_pages, ctx.kv_lens, table, sharing.starts_dev, sharing.pages_dev, sharing.n_groups, sharing.max_members, sharing.shared_bound,
+                             sharing.own_bound, n_heads, scale, status, softcap=softcap, sink=sink, work=work)
     if ctx.is_decode:
         # from the bound; the single lengths have a say only where the step is not captured: a graph is replayed for other lengths
         chunk = decode_chunk_pages(ctx.n_seqs, n_heads, nkv, seen_pages(ctx.kv_len_bound, window, keep, page_size) * page_size, page_size)

@@ -16,9 +16,11 @@ import torch
 
 from ..cache.cache import PAGE_SIZE, SequenceCache
 from ..config import config_from_dict
+from ..csrc import ops
 from ..parts import Runtime
 from ..sampling.sampler import Sampler, SamplingOptions
 from ..weights.random_init import random_tensors
+from .beam import BeamOptions, Hypothesis, beam_loop
 from .generate import GenerationOptions, GenStats, generate_loop
 from .model import build_model, load_model, weight_manifest
 from .graph import GraphDecoder
@@ -117,6 +119,14 @@ class Engine:
     def free_slot(self, slot: int) -> None:
         self._settle()
         self.cache.free_slot(slot)
+
+    def fork_slot(self, slot: int, n: int = 1) -> List[int]:
+        """``n`` new slots that hold the same positions as ``slot`` (all layers, every kind of state); the sequences go on independently.  Full pages of
+        keys and values are shared, a page that is only begun and fixed-size states are copied, in one launch.  CacheFull if there
+        are not enough slots, or pages for the copies; nothing has changed then.  Neighbours in a decode step that share pages have them read once, so
+        give forked slots to ``step`` next to one another."""
+        self._settle()
+        return self.cache.fork([(slot, n)])[0]
 
     def truncate(self, slot: int, n: int) -> None:
         """Keeps the first ``n`` positions of the slot's sequence; the next step's tokens follow them
@@ -219,6 +229,60 @@ class Engine:
         try:
             out, stats = generate_loop(prompts, options, self, stop_token_ids=self.model.spec.stop_token_ids,
                                        on_token=on_token, resume=resume)
+        finally:
+            self._settle()
+        self.last_stats = stats
+        return out
+
+    # -- search over beams ---------------------------------------------------------------------
+    def room_for_beams(self, prompts: Sequence[int], grown: Sequence[int], beams: int) -> bool:
+        """Do requests with prompts of these lengths fit the cache when each has ``beams`` sequences that grow to these lengths behind their shared prompt?"""
+        page = self.cache.page_size
+        need = sum(p // page + beams * (-(-n // page) - p // page) for p, n in zip(prompts, grown))
+        return all(need <= pool.n_free for pool in self.cache.table.pools)
+
+    def fork_slots(self, wanted) -> List[List[int]]:
+        self._settle()
+        return self.cache.fork(wanted)
+
+    def step_and_select(self, slots, tokens, scores, n_out):
+        """One step and the choice behind it.  ``slots``, ``tokens``: all beams' of all requests, a request's next to one another; ``scores``: per request its beams' sums.  Returns per
+        request a list of (score, beam, token), best first."""
+        if self._decoder is not None and all(len(t) == 1 for t in tokens):
+            logits, _ = self._decoder.step(slots, tokens)
+        else:
+            self._settle()
+            logits = self.stepper.step(slots, tokens, "last")
+        outs, row = [], 0
+        sums = torch.tensor([x for s in scores for x in s], dtype=torch.float32).pin_memory().to(logits.device, non_blocking=True)
+        at = 0
+        while at < len(scores):                                 # neighbours with as many beams are one call
+            K, end = len(scores[at]), at
+            while end < len(scores) and len(scores[end]) == K:
+                end += 1
+            rows = (end - at) * K
+            out = torch.empty((3, end - at, n_out), dtype=torch.int32, device=logits.device)
+            ops.beam_select(logits[row:row + rows], sums[row:row + rows].view(end - at, K), n_out, out=out)
+            outs.append(out)
+            row, at = row + rows, end
+        picked = []
+        for out in outs:
+            host = out.cpu()                                    # waits for the step
+            for s, b, v in zip(host[0].view(torch.float32).tolist(), host[1].tolist(), host[2].tolist()):
+                picked.append([x for x in zip(s, b, v) if x[1] >= 0])
+        self.stepper.check_status()
+        return picked
+
+    def beam_search(self, prompts: Sequence[Sequence[int]], options: Optional[BeamOptions] = None, **kw) -> List[List[Hypothesis]]:
+        """Searches for the most probable continuations of every prompt (lists of token ids) with several beams; returns per prompt its ``n_best``
+        hypotheses, best first.  Keyword arguments are ``BeamOptions`` fields.  A prompt is evaluated once; its beams share the pages of what they have in
+        common.  Counters of the run are in ``last_stats``."""
+        if options is None:
+            options = BeamOptions(**kw)
+        elif kw:
+            raise ValueError("give either options or keyword arguments")
+        try:
+            out, stats = beam_loop(prompts, options, self, stop_token_ids=self.model.spec.stop_token_ids)
         finally:
             self._settle()
         self.last_stats = stats

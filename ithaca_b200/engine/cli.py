@@ -5,7 +5,8 @@ Options the reference has keep its names and meanings: ``--model/-m``, ``--promp
 128 generated tokens, three runs after a warm-up of 64, printed as one ``BENCH`` line,
 src/main.cpp:1047-1068).  ``--profile`` stands for the reference's ``ITHACA_PROF`` timers
 (src/model.cpp:1261-1307): it runs the prompts as one step and then one more token each, with
-CUDA events around every kernel call, and prints both steps kernel by kernel.  There is no tokenizer in this library, so a prompt is a list of
+CUDA events around every kernel call, and prints both steps kernel by kernel.  ``--beams`` searches over beams, which the reference
+does not have.  There is no tokenizer in this library, so a prompt is a list of
 token ids (``-p "1,2,3"``); ``-p`` may be given several times for a batch.  After the run
 it prints ``[prompt N tok @ X tok/s | gen M tok @ Y tok/s]`` (src/main.cpp:1140).
 """
@@ -37,6 +38,8 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--top-k", type=int, default=40)
     ap.add_argument("--top-p", type=float, default=0.9)
     ap.add_argument("--rep-pen", type=float, default=1.1, help="repetition penalty over the last 64 generated ids")
+    ap.add_argument("--beams", type=int, default=0, help="search with this many beams for the most probable continuation instead of sampling")
+    ap.add_argument("--length-penalty", type=float, default=1.0, help="with --beams: a hypothesis is ranked by its log probability over its length to this power")
     ap.add_argument("--stop-ids", default=None, help="stop token ids (default: the model's eos_token_id)")
     ap.add_argument("--ctx", "-c", type=int, default=None, help="most positions per sequence (default: the model's)")
     ap.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
@@ -177,8 +180,12 @@ def main(argv: Optional[List[str]] = None) -> int:
         _profile(eng, prompts, args.peaks)
         return 0
     stops = _ids(args.stop_ids) if args.stop_ids is not None else None
-    out = eng.generate(prompts, max_tokens=args.n, temp=args.temp, top_k=args.top_k, top_p=args.top_p,
-                       rep_pen=args.rep_pen, seed=args.seed, stop_token_ids=stops)
+    if args.beams:
+        found = eng.beam_search(prompts, beams=args.beams, max_tokens=args.n, length_penalty=args.length_penalty, stop_token_ids=stops)
+        out = [hyps[0].tokens if hyps else [] for hyps in found]
+    else:
+        out = eng.generate(prompts, max_tokens=args.n, temp=args.temp, top_k=args.top_k, top_p=args.top_p,
+                           rep_pen=args.rep_pen, seed=args.seed, stop_token_ids=stops)
     for o in out:
         print(",".join(str(t) for t in o))
     st = eng.last_stats

@@ -36,6 +36,57 @@ class StepContext:
     host_n_new: List[int] = field(default_factory=list)
     host_kv_lens: List[int] = field(default_factory=list)
     shared: dict = field(default_factory=dict)     # what the layers of one step compute once and share (rotary tables)
+    sharing: List[Optional["Sharing"]] = field(default_factory=list)     # per key/value group: who shares pages (decode steps of forked sequences; else empty)
+
+
+@dataclass
+class Sharing:
+    """Neighbouring sequences of a decode step that share their first pages: group i are the sequences starts[i] <= b < starts[i + 1]."""
+    starts: List[int]
+    pages: List[int]                   # per sequence: pages it shares with its whole group
+    shared_bound: int                  # the most pages a group shares
+    own_bound: int                     # the most pages a sequence has to itself
+    starts_dev: Optional[torch.Tensor] = None
+    pages_dev: Optional[torch.Tensor] = None
+
+    @property
+    def n_groups(self) -> int:
+        return len(self.starts) - 1
+
+    @property
+    def max_members(self) -> int:
+        return max(b - a for a, b in zip(self.starts, self.starts[1:]))
+
+
+def find_sharing(table: np.ndarray, n_pages: Sequence[int]) -> Optional[Sharing]:
+    """``table`` [B, columns]: the block table of a decode step's sequences, ``n_pages``: how many pages each has.  The same page in the same column of
+    neighbouring rows is shared (and full).  Cuts the rows into groups so that the most page readings are saved: m rows that have s first pages in
+    common save (m - 1) s.  None if nothing is shared."""
+    B = table.shape[0]
+    if B < 2:
+        return None
+    common = np.cumprod((table[1:] == table[:-1]) & (table[1:] >= 0), axis=1).sum(axis=1)
+    if not common.any():
+        return None
+
+    # best[j]: the most that rows .. j - 1 save; a group of rows i .. j - 1 adds (j - 1 - i) * min(common[i:j - 1]).  Runs without a common page are told apart first
+    groups = []                                                    # (first row, pages shared)
+    edges = np.concatenate(([0], np.flatnonzero(common == 0) + 1, [B]))
+    for lo, hi in zip(edges[:-1].tolist(), edges[1:].tolist()):
+        best, cuts = np.zeros(hi - lo + 1, dtype=np.int64), [(0, 0)] * (hi - lo + 1)
+        for j in range(1, hi - lo + 1):
+            least = np.concatenate((np.minimum.accumulate(common[lo:lo + j - 1][::-1])[::-1], [0]))       # of rows i .. j - 1, for every i
+            gain = best[:j] + np.arange(j - 1, -1, -1) * least
+            i = int(gain.argmax())                                 # of equal ways the larger group
+            best[j], cuts[j] = gain[i], (i, int(least[i]))
+        at, found = hi - lo, []
+        while at > 0:
+            at, least_here = cuts[at]
+            found.append((lo + at, least_here))
+        groups += found[::-1]
+    starts = [g[0] for g in groups] + [B]
+    pages = [s for (a, s), b in zip(groups, starts[1:]) for _ in range(b - a)]
+    return Sharing(starts, pages, max(pages), max(n - s for n, s in zip(n_pages, pages)))
 
 
 def field_offsets(sizes):
@@ -65,11 +116,11 @@ class ContextBuilder:
 
     def build(self, slots: Sequence[int], tokens: Sequence[Sequence[int]], start: Sequence[int],
               want: Sequence[Sequence[int]], tables: Sequence[np.ndarray],
-              into: Optional[torch.Tensor] = None) -> StepContext:
+              into: Optional[torch.Tensor] = None, sharing: Sequence[Optional[Sharing]] = ()) -> StepContext:
         """``start[b]``: positions sequence b holds before the step.  ``tables[g]``: the
         [B, pages] block table of group g (pages already reserved for the new tokens).
         ``into``: a device buffer to fill instead of a fresh one (its layout must be the
-        same as at its first use; CUDA graphs replay on it)."""
+        same as at its first use; CUDA graphs replay on it).  ``sharing``: per group, who shares pages."""
         B = len(slots)
         n_new = [len(t) for t in tokens]
         T = int(sum(n_new))
@@ -82,6 +133,7 @@ class ContextBuilder:
         kv_lens = np.asarray(start, dtype=np.int32) + np.asarray(n_new, dtype=np.int32)
         parts = [token_ids, token_seq, token_pos, cu, np.asarray(slots, dtype=np.int32), kv_lens, rows]
         parts += [np.ascontiguousarray(t, dtype=np.int32).reshape(-1) for t in tables]
+        parts += [np.asarray(x, dtype=np.int32) for s in sharing if s is not None for x in (s.starts, s.pages)]
         offs, sizes, total = field_offsets([p.size for p in parts])
         if self._copied is not None:
             self._copied.synchronize()                        # the staging buffer is free again
@@ -104,10 +156,14 @@ class ContextBuilder:
         def view(i):
             return dev[offs[i]:offs[i] + sizes[i]]
 
+        at = 7 + len(tables)
+        for s in sharing:
+            if s is not None:
+                s.starts_dev, s.pages_dev, at = view(at), view(at + 1), at + 2
         tabs = [view(7 + g).view(B, tables[g].shape[1]) for g in range(len(tables))]
         return StepContext(
             n_tokens=T, n_seqs=B, n_logit_rows=int(rows.size), token_ids=view(0), token_seq=view(1),
             token_pos=view(2), cu_seqlens=view(3), slots=view(4), kv_lens=view(5), logit_rows=view(6), tables=tabs,
             is_decode=all(n == 1 for n in n_new), max_new=max(n_new) if n_new else 0,
             max_kv_len=int(kv_lens.max()) if B else 0, kv_len_bound=int(kv_lens.max()) if B else 0, host_slots=list(slots), host_n_new=n_new,
-            host_kv_lens=[int(x) for x in kv_lens])
+            host_kv_lens=[int(x) for x in kv_lens], sharing=list(sharing))

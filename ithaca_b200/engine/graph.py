@@ -4,7 +4,7 @@ A decode step is some hundreds of small launches; issued one by one from Python
 they cost more than the step itself.  The reference captures its whole
 single-token forward into one graph and replays it, reading the position from
 device memory (src/model.cpp:1341-1350, src/cuda_tier.cpp:630-651).  Here a graph
-is captured per (number of sequences, block-table width): the step's description
+is captured per (number of sequences, block-table width, and where sequences share pages how they do): the step's description
 (tokens, positions, lengths, block tables) lives in one device buffer that is
 refilled before each replay, so the same graph serves every step of that shape.
 The graph covers the forward pass, the greedy pick, and a copy of the kernels'
@@ -32,7 +32,7 @@ import torch
 
 from ..cache.pages import CacheError
 from ..csrc import ops
-from .context import StepContext, field_offsets
+from .context import Sharing, field_offsets
 from .step import StepError, Stepper
 
 
@@ -76,10 +76,16 @@ def _bucket(cols: int) -> int:
     return -(-cols // step) * step
 
 
+def _sharing_shape(f: Optional[Sharing]):
+    """What a captured step takes from who shares pages: the number of groups, the largest, and bounds of the pages shared and not (rounded up, so
+    that growing sequences re-capture rarely)."""
+    return None if f is None else (f.n_groups, f.max_members, _bucket(f.shared_bound), _bucket(f.own_bound))
+
+
 class GraphDecoder:
     def __init__(self, stepper: Stepper):
         self.stepper = stepper
-        self.graphs: Dict[Tuple[int, int], _Captured] = {}
+        self.graphs: Dict[tuple, _Captured] = {}
         self.launches_last_step = 0
         self.last_upload_bytes = 0
         self._ahead: Optional[_Launched] = None          # the step launched before its tokens reached the host
@@ -186,12 +192,16 @@ class GraphDecoder:
             if int(lens.max()) + 1 > st.max_position:
                 raise StepError(f"a sequence would exceed the model's limit of {st.max_position} positions")
             cols = _bucket(int(-(-(int(lens.max()) + 1) // page)))
-            cap = self.graphs.get((B, cols))
+            sharing = []
+            if any(pool.n_shared for pool in table.pools):
+                sharing = st.sharing([t[idx, :cols] for t in table.tables], (lens // page + 1).tolist())
+            key = (B, cols) + tuple(_sharing_shape(f) for f in sharing)
+            cap = self.graphs.get(key)
             if cap is None:
                 if tokens is None:
                     return None                               # a new shape is captured with real tokens only
                 cap = self._capture(slots, [[t] for t in tokens], cols)
-                self.graphs[(B, cols)] = cap
+                self.graphs[key] = cap
                 self.launches_last_step = cap.launches
                 return cap
             # pages: a sequence needs a new one only when it stands at a page boundary
@@ -212,13 +222,13 @@ class GraphDecoder:
             sn[o[0]:o[0] + B] = toks
         sn[o[2]:o[2] + B] = lens
         sn[o[5]:o[5] + B] = lens + 1
-        key = tuple(slots)
-        if cap.stage_slots[k] != key:
+        order = tuple(slots)
+        if cap.stage_slots[k] != order:
             sn[o[1]:o[1] + B] = np.arange(B)
             sn[o[3]:o[3] + B + 1] = np.arange(B + 1)
             sn[o[4]:o[4] + B] = idx
             sn[o[6]:o[6] + B] = np.arange(B)
-            cap.stage_slots[k] = key
+            cap.stage_slots[k] = order
         for g in range(len(st.cache.kv_groups)):
             t = table.tables[g]
             dst = sn[o[7 + g]:o[7 + g] + B * cols].reshape(B, cols)
@@ -226,6 +236,12 @@ class GraphDecoder:
             dst[:, :c] = t[idx, :c]
             if c < cols:
                 dst[:, c:] = -1
+        n = 7 + len(st.cache.kv_groups)
+        for f in sharing:
+            if f is not None:
+                sn[o[n]:o[n] + len(f.starts)] = f.starts
+                sn[o[n + 1]:o[n + 1] + B] = f.pages
+                n += 2
         cap.buffer.copy_(cap.stages[k], non_blocking=True)
         if cap.stage_events[k] is None:
             cap.stage_events[k] = torch.cuda.Event()
@@ -251,9 +267,15 @@ class GraphDecoder:
         page = st.cache.page_size
         B = len(slots)
         n_groups = len(st.cache.kv_groups)
-        offsets, sizes, total = field_offsets([B, B, B, B + 1, B, B, B] + [B * cols] * n_groups)
-        buffer = torch.empty(total, dtype=torch.int32, device=st.runtime.device)
+        # room for who shares pages: up to B groups in every key/value group (the buffer may be longer than what it describes)
+        room = field_offsets([B, B, B, B + 1, B, B, B] + [B * cols] * n_groups + [B + 1, B] * n_groups)[2]
+        buffer = torch.empty(room, dtype=torch.int32, device=st.runtime.device)
         ctx = st.prepare(slots, tokens, "last", into=buffer, table_cols=cols)
+        sharing = [f for f in ctx.sharing if f is not None]
+        offsets, sizes, total = field_offsets([B, B, B, B + 1, B, B, B] + [B * cols] * n_groups + [n for f in sharing for n in (len(f.starts), B)])
+        buffer = buffer[:total]
+        for f in sharing:                                     # as for the lengths: sizes of grids follow from the shape the graph is kept under
+            _, _, f.shared_bound, f.own_bound = _sharing_shape(f)
         # the graph is replayed for other lengths: what the kernels choose for it follows from its shape alone, not from which lengths came first
         ctx.kv_len_bound, ctx.replayed = cols * page, True
         torch.cuda.current_stream().synchronize()

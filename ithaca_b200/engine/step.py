@@ -19,7 +19,7 @@ import torch
 
 from ..cache.cache import SequenceCache
 from ..cache.pages import CacheError
-from .context import ContextBuilder, StepContext
+from .context import ContextBuilder, Sharing, StepContext, find_sharing
 
 
 class StepError(ValueError):
@@ -92,7 +92,25 @@ class Stepper:
                 raise StepError("the block table is narrower than the longest sequence")
             cols = table_cols
         tables = [self.cache.table.table_rows(g, slots, cols) for g in range(len(self.cache.kv_groups))]
-        return self.builder.build(slots, tokens, start, want_lists, tables, into=into)
+        sharing = self.sharing(tables, [-(-(st + 1) // page) for st in start]) if all(n == 1 for n in n_new) else ()
+        return self.builder.build(slots, tokens, start, want_lists, tables, into=into, sharing=sharing)
+
+    def sharing(self, tables: Sequence[np.ndarray], n_pages: Sequence[int]) -> List[Optional[Sharing]]:
+        """Per key/value group which neighbours of a decode step share pages, where a kernel reads such pages once; an empty list if there are none.  ``tables``:
+        the step's block tables, ``n_pages``: the pages of each sequence."""
+        out: List[Optional[Sharing]] = []
+        if self.runtime.dtype != "bfloat16" or not any(pool.n_shared for pool in self.cache.table.pools):
+            return out
+        from ..csrc import attention_bf16
+        for grp, pool, t in zip(self.cache.kv_groups, self.cache.table.pools, tables):
+            found = None
+            if (pool.n_shared and grp.window is None and not grp.key_scales and grp.v_head_dim in (None, grp.head_dim) and self.cache.page_size == 64
+                    and attention_bf16.supported(grp.head_dim)):
+                found = find_sharing(t, n_pages)
+                if found is not None and not attention_bf16.sharing_pays(found.starts, found.pages, n_pages, grp.n_kv_heads, grp.head_dim):
+                    found = None
+            out.append(found)
+        return out if any(f is not None for f in out) else []
 
     def finish(self, ctx: StepContext) -> None:
         self.cache.commit(ctx.host_slots, ctx.host_n_new)

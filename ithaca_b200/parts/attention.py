@@ -306,8 +306,10 @@ def attend(q: torch.Tensor, cache: LayerCache, ctx, table: torch.Tensor, n_heads
     rows that are keys and values."""
     if q.dtype == torch.bfloat16 and (cache.v_pages is None or cache.v_pages.shape[3] == cache.k_pages.shape[3]):
         from ..csrc import attention_bf16
+        sharing = getattr(ctx, "sharing", None)
         out = attention_bf16.attend(q, cache.k_pages, cache.v_pages, ctx, table, n_heads, scale, window, rt.status,
-                                    softcap=softcap, sink=sink, keep=keep, key_scales=cache.key_scales, slopes=slopes, reach=reach)
+                                    softcap=softcap, sink=sink, keep=keep, key_scales=cache.key_scales, slopes=slopes, reach=reach,
+                                    sharing=sharing[cache.kv_group] if sharing else None)
         if out is not None:
             return out
     plain = not torch.is_tensor(sink) and not (sink or softcap or keep) and cache.key_scales is None and slopes is None
