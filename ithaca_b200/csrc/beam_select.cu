@@ -2,19 +2,16 @@
 // row of logits l[r,b,:].  A candidate (b, v) scores c[r,b] + (l[r,b,v] - lse[r,b]) with lse[r,b] = log sum_v exp l[r,b,v]; the n
 // largest of a request are wanted in descending order, equal ones by ascending b V + v.
 //
-// One pass over the logits.  Slices of a row go to blocks of their own (beam_rows_kernel): a block keeps its slice in registers, forms the
-// slice's maximum and sum of exponentials, and finds its n largest logits; within a row the order of the logits is the order of the
-// scores, so only those can be among a request's n best.  A second kernel (beam_merge_kernel, a block per request) joins the slices' sums into
-// the beams' lse and picks from the lists.
-//
-// Finding the n largest without a sort: of the threads' own largest elements (every thread holds up to 32), the n-th largest, tau, is a lower
-// bound of the slice's n-th largest, and only the n threads whose largest is at least tau hold elements >= tau.  So at most 32 n
-// elements are gathered, whatever the data, and usually hardly more than n; their ranks are counted.  An element's key is its value (as an integer that
-// orders like the value) above its place's complement, so keys are distinct and equal values come by ascending place.  The merge does the same with
-// the lists: the n-th largest head is a bound, and only n lists have entries above it.
+// One pass over the logits and a second look at small pieces of them, no sort.  beam_tiles_kernel: a warp takes a tile of 1,024 logits of a row and leaves
+// the tile's maximum, where it stands, the one behind it, and the sum of exponentials below it.  beam_merge_kernel, a block per request: joins the
+// sums into the beams' lse, and with them every tile's maximum into a score.  Of these the n-th largest is a lower bound of the n-th best candidate (n tiles
+// have a candidate at least as good), and only tiles that are not below it can hold any of the n best: hardly more than n.  Of a tile whose second largest is below the
+// bound the maximum is all that counts; the others are read again (L2 has them) for what is not below it.  What is gathered, usually hardly more than n, is
+// ranked by counting.  A tile gives at most n: one that has more (sorted or constant logits) gives its n best one at a time; where many tiles are as good as the
+// bound, the n best are found by exact comparisons with their places.
 //
 // Scores are formed and compared in 64 bits (two beams' candidates may be closer than a float of their size can tell) and rounded once;
-// exponentials are floats, summed in float over 32 terms and in 64 bits beyond.  A logit of -inf or NaN is no candidate; neither is any of a beam
+// exponentials are floats, summed in float within a tile and in 64 bits beyond.  A logit of -inf or NaN is no candidate; neither is any of a beam
 // whose sum is -inf or NaN.  Where a row has logits of +inf, they share the probability.  Places without a candidate: score -inf, beam and token -1.
 #include <math.h>
 #define IK_FAMILY 16
@@ -22,243 +19,349 @@
 
 namespace {
 
-typedef unsigned long long u64;
+constexpr int TILE = 1024, PER = TILE / 32;                            // logits of a tile, of a lane
+constexpr int RT = 256, MT = 512, MW = MT / 32;                        // threads of the two kernels
+constexpr int BEAMS = 16, OUT = 32, TILES = 1024;                      // most beams, results and tiles of a row
+constexpr int PICKS = 40;                                              // tiles that the merge takes as they come
 
-constexpr int BT = 256, BE = 32, SLICE = BT * BE;                    // threads, elements of a thread and of a block
-constexpr int BEAMS = 16, OUT = 32, SLICES = 128;                    // most beams, results and slices of a row
+// What a tile leaves: its maximum, the one behind it (equal to it where it stands twice), the sum of exponentials below the maximum; the maximum's place in its row and the
+// beam in the upper 12 bits.
+struct __align__(16) Tile { float top, second, sum; uint32_t where; };
+static_assert(TILES * TILE <= 1 << 20 && BEAMS <= 1 << 12, "a place and a beam share 32 bits");
+__device__ __forceinline__ uint32_t place_of(const Tile& t) { return t.where & 0xfffffu; }
+__device__ __forceinline__ int beam_of(const Tile& t) { return (int)(t.where >> 20); }
 
-__device__ __forceinline__ uint32_t order_key(float v) {
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// A lane's logits of a tile that starts at `lo`; what lies behind the row is -inf.  VEC: rows on 16 bytes of a multiple of four logits.  The order in which a
+// tile is summed does not depend on where it lies in memory, so equal rows give equal sums and equal candidates stay equal.
+template <bool VEC> __device__ __forceinline__ int place_in(int e, int lane) { return VEC ? (e >> 2) * 128 + lane * 4 + (e & 3) : e * 32 + lane; }
+template <bool VEC>
+__device__ __forceinline__ void load_tile(float (&v)[PER], const float* __restrict__ w, int lo, int V, int lane) {
+    if (VEC) {
+        #pragma unroll
+        for (int i = 0; i < PER / 4; i++) {
+            const int at = lo + place_in<true>(4 * i, lane);
+            const float4 x = at < V ? *reinterpret_cast<const float4*>(w + at) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            v[4 * i] = x.x; v[4 * i + 1] = x.y; v[4 * i + 2] = x.z; v[4 * i + 3] = x.w;
+        }
+    } else {
+        #pragma unroll
+        for (int e = 0; e < PER; e++) v[e] = lo + e * 32 + lane < V ? w[lo + e * 32 + lane] : -INFINITY;
+    }
+}
+
+template <bool VEC>
+__global__ void __launch_bounds__(RT, 5)
+beam_tiles_kernel(const float* __restrict__ logits, long long ldl, const float* __restrict__ sums, int K, int V, int tiles, Tile* __restrict__ out) {
+    ik_pdl_wait();
+    ik_pdl_launch_dependents();
+    const int lane = threadIdx.x & 31, row = blockIdx.x, tile = blockIdx.y * (RT / 32) + (threadIdx.x >> 5);
+    if (tile >= tiles) return;
+    const int lo = tile * TILE, beam = row % K;
+    if (!(sums[row] > -INFINITY)) {                                    // a dead beam: not read
+        if (lane == 0) out[(size_t)row * tiles + tile] = Tile{-INFINITY, -INFINITY, 0.f, (uint32_t)beam << 20 | (uint32_t)lo};
+        return;
+    }
+    float v[PER];
+    load_tile<VEC>(v, logits + (long long)row * ldl, lo, V, lane);
+    constexpr int GROUPS = 4, IN = PER / GROUPS;
+    float group[GROUPS], top = -INFINITY;
+    #pragma unroll
+    for (int g = 0; g < GROUPS; g++) {
+        group[g] = -INFINITY;
+        #pragma unroll
+        for (int e = 0; e < IN; e++) group[g] = fmaxf(group[g], v[g * IN + e]);       // (the other operand where one is NaN)
+        top = fmaxf(top, group[g]);
+    }
+    #pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    // where the maximum stands first, how often, and what comes behind it: only the groups that have it are looked through
+    int first = TILE, times = 0;
+    float second = -INFINITY;
+    #pragma unroll
+    for (int g = GROUPS - 1; g >= 0; g--)
+        if (__any_sync(0xffffffffu, group[g] == top)) {
+            #pragma unroll
+            for (int e = IN - 1; e >= 0; e--) {
+                const bool is = v[g * IN + e] == top;
+                first = is ? place_in<VEC>(g * IN + e, lane) : first;
+                times += is;
+                second = fmaxf(second, is ? -INFINITY : v[g * IN + e]);
+            }
+        } else second = fmaxf(second, group[g]);
+    #pragma unroll
+    for (int o = 16; o > 0; o >>= 1) second = fmaxf(second, __shfl_xor_sync(0xffffffffu, second, o));
+    if (__reduce_add_sync(0xffffffffu, times) > 1) second = top;
+    first = __reduce_min_sync(0xffffffffu, first);
+    float s = 0.f;
+    if (top < INFINITY) {
+        // the difference first, then the factor: a product with -top log2 e inside would carry one rounding error into all terms.  The bound keeps NaN and
+        // -inf out of the sum (2^-150 is 0)
+        #pragma unroll
+        for (int e = 0; e < PER; e++) s += ex2(fmaxf((v[e] - top) * 1.4426950408889634f, -150.f));
+    } else {
+        #pragma unroll
+        for (int e = 0; e < PER; e++) s += v[e] == INFINITY ? 1.f : 0.f;
+    }
+    #pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (lane == 0) out[(size_t)row * tiles + tile] = Tile{top, second, s, (uint32_t)beam << 20 | (uint32_t)(lo + first)};
+}
+
+// A candidate: its score as an integer that orders like it, and its place (beam * V + token); no candidate: 0 and NOWHERE.  Ordered by descending scores, equal ones by
+// ascending place.  Compared without branches: a warp that jumps at every comparison takes 190 cycles for one step of a ranking, without jumps a tenth of that.
+struct __align__(16) Cand { unsigned long long s; uint32_t at; };
+constexpr uint32_t NOWHERE = 0xffffffffu;
+__device__ __forceinline__ Cand none() { return Cand{0ull, NOWHERE}; }
+__device__ __forceinline__ unsigned long long order_key(double v) {    // more than 0
+    const long long b = __double_as_longlong(v);
+    return (unsigned long long)(b ^ ((b >> 63) | (long long)0x8000000000000000ull));
+}
+__device__ __forceinline__ double order_value(unsigned long long k) {
+    return __longlong_as_double((long long)(k ^ ((k >> 63) ? 0x8000000000000000ull : ~0ull)));
+}
+__device__ __forceinline__ bool ahead(const Cand& a, const Cand& b) { return (a.s > b.s) | ((a.s == b.s) & (a.at < b.at)); }
+__device__ __forceinline__ Cand shfl_xor(const Cand& c, int m) { return Cand{__shfl_xor_sync(0xffffffffu, c.s, m), __shfl_xor_sync(0xffffffffu, c.at, m)}; }
+__device__ __forceinline__ Cand pick(bool second, const Cand& a, const Cand& b) { return Cand{second ? b.s : a.s, second ? b.at : a.at}; }
+__device__ __forceinline__ Cand better(const Cand& a, const Cand& b) { return pick(ahead(b, a), a, b); }
+
+__device__ __forceinline__ float shfl_xor(float c, int m) { return __shfl_xor_sync(0xffffffffu, c, m); }
+__device__ __forceinline__ float exchange(bool front, float mine, float other) { return front ? fmaxf(mine, other) : fminf(mine, other); }
+__device__ __forceinline__ Cand exchange(bool front, const Cand& mine, const Cand& other) { return pick(front == ahead(other, mine), mine, other); }
+__device__ __forceinline__ float better(float a, float b) { return fmaxf(a, b); }
+__device__ __forceinline__ uint32_t order_key(float v) {               // orders like the value; more than 0
     const uint32_t b = __float_as_uint(v);
     return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
-__device__ __forceinline__ float order_value(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k); }
-__device__ __forceinline__ u64 key_of(float v, uint32_t at) { return ((u64)order_key(v) << 32) | (uint32_t)~at; }
 
-__device__ __forceinline__ u64 shfl_xor64(u64 v, int m) { return __shfl_xor_sync(0xffffffffu, v, m); }
-
-// A warp's 32 keys in descending order (lane 0 the largest): bitonic.
-__device__ __forceinline__ u64 warp_sort_desc(u64 k, int lane) {
+// A warp's 32 candidates (or floats) in order, lane 0 the best: bitonic.
+template <typename T>
+__device__ __forceinline__ T warp_sort(T k, int lane) {
     #pragma unroll
     for (int size = 2; size <= 32; size <<= 1)
         #pragma unroll
         for (int step = size >> 1; step > 0; step >>= 1) {
-            const u64 o = shfl_xor64(k, step);
-            const bool up = (lane & size) == 0, first = (lane & step) == 0;     // up: descending half
-            k = (up == first) ? (k > o ? k : o) : (k < o ? k : o);
+            const T o = shfl_xor(k, step);
+            const bool front = ((lane & size) == 0) == ((lane & step) == 0);
+            k = exchange(front, k, o);
         }
     return k;
 }
-// Of two such lists the 32 largest, in order: the larger of a[i] and b[31 - i] are those, as a bitonic sequence.
-__device__ __forceinline__ u64 warp_merge_desc(u64 a, u64 b_reversed, int lane) {
-    u64 k = a > b_reversed ? a : b_reversed;
+// The best 32 of two sorted lists, in order: the better of a[i] and b[31 - i] are those, as a bitonic sequence.
+template <typename T>
+__device__ __forceinline__ T warp_merge(T a, const T& b_reversed, int lane) {
+    a = better(a, b_reversed);
     #pragma unroll
     for (int step = 16; step > 0; step >>= 1) {
-        const u64 o = shfl_xor64(k, step);
-        k = ((lane & step) == 0) ? (k > o ? k : o) : (k < o ? k : o);
+        const T o = shfl_xor(a, step);
+        const bool front = (lane & step) == 0;
+        a = exchange(front, a, o);
     }
-    return k;
+    return a;
 }
 
-// scratch: keys [rows][slices][n], then (maximum, sum) [rows][slices] as doubles
-__global__ void __launch_bounds__(BT)
-beam_rows_kernel(const float* __restrict__ logits, long long ldl, const float* __restrict__ sums, int V, int n, int slices,
-                 u64* __restrict__ keys, double2* __restrict__ stats) {
-    __shared__ u64 sorted[BT / 32][32];
-    __shared__ u64 cand[OUT * BE];
-    __shared__ float red_m[BT / 32];
-    __shared__ double red_s[BT / 32];
-    __shared__ int n_cand;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int row = blockIdx.x, slice = blockIdx.y;
-    u64* const out = keys + ((size_t)row * slices + slice) * n;
-    if (!(sums[row] > -INFINITY)) return;                              // a dead beam: the merge does not look at its lists
-    const float* const w = logits + (long long)row * ldl;
-    const int per = (V + slices - 1) / slices, lo = slice * per, hi = min(V, lo + per);
-    // element e of a thread stands at lo + e BT + tid, whatever the row's alignment: equal rows give equal sums, so that equal candidates stay equal
-    float v[BE];
-    #pragma unroll
-    for (int e = 0; e < BE; e++) v[e] = lo + e * BT + tid < hi ? w[lo + e * BT + tid] : -INFINITY;
-    float m = -INFINITY;
-    #pragma unroll
-    for (int e = 0; e < BE; e++) {
-        v[e] = v[e] > -INFINITY ? v[e] : -INFINITY;                    // NaN too
-        m = fmaxf(m, v[e]);
-    }
-    // the thread's largest, the first of equals
-    int best = 0;
-    #pragma unroll
-    for (int e = BE - 1; e >= 0; e--) best = v[e] == m ? e : best;
-    auto place = [&](int e) { return (uint32_t)(lo + e * BT + tid); };
-    const u64 mine = m > -INFINITY ? key_of(m, place(best)) : 0ull;
-    u64 k = warp_sort_desc(mine, lane);
-    sorted[warp][lane] = k;
-    float mm = m;
-    #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
-    if (lane == 0) red_m[warp] = mm;
-    if (tid == 0) n_cand = 0;
-    __syncthreads();
-    #pragma unroll
-    for (int i = 0; i < BT / 32; i++) mm = fmaxf(mm, red_m[i]);
-    // the slice's sum of exponentials (elements equal to the maximum count 1, an infinite one too)
-    float s = 0.f;
-    #pragma unroll
-    for (int e = 0; e < BE; e++) s += v[e] == mm ? 1.0f : expf(v[e] - mm);
-    double ss = mm > -INFINITY ? (double)s : 0.0;
-    #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    if (lane == 0) red_s[warp] = ss;
-    // the 32 largest of the threads' largest
-    #pragma unroll
-    for (int half = BT / 64; half > 0; half >>= 1) {
-        if (warp < half) k = warp_merge_desc(k, sorted[warp + half][31 - lane], lane);
-        __syncthreads();
-        if (warp < half) sorted[warp][lane] = k;
-        __syncthreads();
-    }
-    if (tid == 0) {
-        double t = 0.0;
-        for (int i = 0; i < BT / 32; i++) t += red_s[i];
-        stats[(size_t)row * slices + slice] = make_double2((double)mm, t);
-    }
-    const u64 tau = max(sorted[0][n - 1], 1ull);
-    if (mine >= tau) {
-        #pragma unroll
-        for (int e = 0; e < BE; e++)
-            if (v[e] > -INFINITY) {
-                const u64 c = key_of(v[e], place(e));
-                if (c >= tau) cand[atomicAdd(&n_cand, 1)] = c;        // at most n threads come here: never more than n BE
-            }
-    }
-    __syncthreads();
-    const int c = n_cand;
-    for (int i = tid; i < c; i += BT) {
-        const u64 me = cand[i];
-        int rank = 0;
-        for (int j = 0; j < c; j++) rank += cand[j] > me;
-        if (rank < n) out[rank] = me;
-    }
-    for (int i = c + tid; i < n; i += BT) out[i] = 0ull;
+// How many of a list are ahead of its i-th (a warp).
+__device__ __forceinline__ int rank_of(const Cand* list, int count, int i, int lane) {
+    const Cand me = list[i];
+    int rank = 0;
+    for (int j = lane; j < count; j += 32) rank += ahead(list[j], me) ? 1 : 0;
+    return __reduce_add_sync(0xffffffffu, rank);
 }
 
-// A candidate of the merge: descending scores, equal ones by ascending place (beam * V + token).
-__device__ __forceinline__ bool ahead(double s, uint32_t at, double s2, uint32_t at2) { return s > s2 || (s == s2 && at < at2); }
+// What the merge keeps of a beam: its sum (-inf: nothing to choose), its lse, whether infinite logits share its probability.
+struct Beam { double base, lse; int shares; };
+__device__ __forceinline__ double score_of(const Beam& b, float l) {
+    if (b.shares) l = l < INFINITY ? -INFINITY : 0.f;
+    const double s = b.base + ((double)l - b.lse);
+    return l > -INFINITY ? s : -(double)INFINITY;                      // (a dead beam's sum is -inf, too)
+}
+__device__ __forceinline__ Cand cand_of(const Beam& b, float l, uint32_t at) {
+    const double s = score_of(b, l);
+    return pick(s > -INFINITY, none(), Cand{order_key(s), at});
+}
 
-__global__ void __launch_bounds__(BT)
-beam_merge_kernel(const u64* __restrict__ keys, const double2* __restrict__ stats, const float* __restrict__ sums, int K, int V, int n, int slices,
+template <bool VEC>
+__global__ void __launch_bounds__(MT, 1)
+beam_merge_kernel(const float* __restrict__ logits, long long ldl, const Tile* __restrict__ tile_of, const float* __restrict__ sums, int K, int V, int n, int tiles,
                   float* __restrict__ out_s, int* __restrict__ out_b, int* __restrict__ out_v) {
-    extern __shared__ __align__(16) unsigned char smem[];
-    const int lists = K * slices;
-    double* const head_s = reinterpret_cast<double*>(smem);            // [lists]
-    uint32_t* const head_at = reinterpret_cast<uint32_t*>(head_s + lists);
-    __shared__ double cand_s[OUT * OUT];
-    __shared__ uint32_t cand_at[OUT * OUT];
-    __shared__ int picked[OUT];
-    __shared__ double lse[BEAMS], base[BEAMS];
-    __shared__ int shares[BEAMS];                                      // a beam with infinite logits
-    __shared__ int n_picked, n_cand, tau_list;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int r = blockIdx.x;
-    for (int b = warp; b < K; b += BT / 32) {
+    __shared__ Beam beams[BEAMS];
+    __shared__ float sorted[2 * MW][32];                               // lists of the merge's levels, one behind the other
+    __shared__ Cand cand[PICKS * OUT], picked[OUT * 32];               // candidates; tiles by their maxima
+    __shared__ int picked_tile[OUT * 32], chosen[PICKS];
+    __shared__ int n_picked, n_cand;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = blockIdx.x, total = K * tiles;
+    if (tid == 0) n_picked = n_cand = 0;
+    ik_pdl_wait();
+    IK_AFTER_WAIT(tile_of);
+    IK_AFTER_WAIT(sums);
+    IK_AFTER_WAIT(logits);
+    const Tile* const mine = tile_of + (size_t)r * total;
+    for (int b = warp; b < K; b += MW) {
         const float c = sums[r * K + b];
-        const bool live = c > -INFINITY;
-        double m = -INFINITY, s = 0.0;
-        if (live) {
-            for (int i = lane; i < slices; i += 32) m = fmax(m, stats[(size_t)(r * K + b) * slices + i].x);
-            #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) m = fmax(m, __shfl_xor_sync(0xffffffffu, m, o));
-            for (int i = lane; i < slices; i += 32) {
-                const double2 t = stats[(size_t)(r * K + b) * slices + i];
-                s += t.x == m ? t.y : t.y * exp(t.x - m);
-            }
-            #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        }
+        const Tile* const row = mine + b * tiles;
+        float top = -INFINITY;
+        double s = 0.0;
+        #pragma unroll 4
+        for (int i = lane; i < tiles; i += 32) top = fmaxf(top, row[i].top);
+        #pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        #pragma unroll 4
+        for (int i = lane; i < tiles; i += 32) s += (double)(row[i].top == top ? row[i].sum : row[i].sum * expf(row[i].top - top));
+        #pragma unroll
+        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
         if (lane == 0) {
-            const bool any = live && m > -INFINITY, inf = m == INFINITY;
-            base[b] = any ? (double)c : -INFINITY;
-            lse[b] = any ? (inf ? log(s) : m + log(s)) : 0.0;
-            shares[b] = inf;
+            const bool any = top > -INFINITY, inf = top == INFINITY;
+            beams[b] = Beam{any ? (double)c : -(double)INFINITY, any ? (inf ? log(s) : (double)top + log(s)) : 0.0, inf};
         }
     }
-    if (tid == 0) { n_picked = n_cand = 0; tau_list = -1; }
     __syncthreads();
-    auto score = [&](int b, u64 key) {                                 // -inf: not a candidate
-        if (key == 0ull || !(base[b] > -INFINITY)) return -(double)INFINITY;
-        double l = (double)order_value((uint32_t)(key >> 32));
-        if (shares[b]) { if (l < INFINITY) return -(double)INFINITY; l = 0.0; }
-        return base[b] + (l - lse[b]);
+    auto tile_cand = [&](int i) {
+        const Tile t = mine[i];
+        return cand_of(beams[beam_of(t)], t.top, (uint32_t)beam_of(t) * (uint32_t)V + place_of(t));
     };
-    auto place = [&](int b, u64 key) { return (uint32_t)b * (uint32_t)V + (uint32_t)~(uint32_t)key; };
-    for (int i = tid; i < lists; i += BT) {
-        const int b = i / slices;
-        const u64 key = base[b] > -INFINITY ? keys[((size_t)r * lists + i) * n] : 0ull;
-        head_s[i] = score(b, key);
-        head_at[i] = head_s[i] > -INFINITY ? place(b, key) : 0xffffffffu - i;
+    // a bound from the threads' best tiles.  Rounded to float the order stays (but for ties), so the n-th largest float is that of the n-th best, and the tiles
+    // that are not below it are few: at most n threads have any, unless many are as good as equal
+    float best = -INFINITY;
+    for (int i = tid; i < total; i += MT) {
+        const Tile t = mine[i];
+        best = fmaxf(best, (float)score_of(beams[beam_of(t)], t.top));
+    }
+    float k = warp_sort(best, lane);
+    sorted[warp][lane] = k;
+    #pragma unroll 1
+    for (int half = MW / 2; half > 0; half >>= 1) {
+        __syncthreads();
+        if (warp < half) {
+            k = warp_merge(k, sorted[2 * MW - 4 * half + warp + half][31 - lane], lane);
+            sorted[2 * MW - 2 * half + warp][lane] = k;
+        }
     }
     __syncthreads();
-    if (lists > n)                                                      // the n-th largest head
-        for (int i = tid; i < lists; i += BT) {
-            const double s = head_s[i];
-            const uint32_t at = head_at[i];
-            int rank = 0;
-            for (int j = 0; j < lists; j++) rank += ahead(head_s[j], head_at[j], s, at);
-            if (rank == n - 1) tau_list = i;
+    const float bound = sorted[2 * MW - 2][n - 1];
+    if (best > -INFINITY && best >= bound)
+        for (int i = tid; i < total; i += MT) {
+            const Cand c = tile_cand(i);
+            if (c.s && (float)order_value(c.s) >= bound) {
+                const int at = atomicAdd(&n_picked, 1);
+                if (at < PICKS) { picked[at] = c; picked_tile[at] = i; }
+            }
         }
     __syncthreads();
-    const double tau_s = tau_list < 0 ? -(double)INFINITY : head_s[tau_list];
-    const uint32_t tau_at = tau_list < 0 ? 0xffffffffu : head_at[tau_list];
-    for (int i = tid; i < lists; i += BT)
-        if (head_s[i] > -INFINITY && !ahead(tau_s, tau_at, head_s[i], head_at[i])) picked[atomicAdd(&n_picked, 1)] = i;
+    int p = n_picked;
+    if (p > PICKS) {                                                   // many equal ones: the bound from the exact order
+        Cand mine_best = none();
+        for (int i = tid; i < total; i += MT) mine_best = better(mine_best, tile_cand(i));
+        Cand kc = warp_sort(mine_best, lane);
+        if (tid == 0) n_picked = 0;
+        cand[warp * 32 + lane] = kc;
+        #pragma unroll 1
+        for (int half = MW / 2; half > 0; half >>= 1) {
+            __syncthreads();
+            if (warp < half) kc = warp_merge(kc, cand[(warp + half) * 32 + 31 - lane], lane);
+            __syncthreads();
+            if (warp < half) cand[warp * 32 + lane] = kc;
+        }
+        __syncthreads();
+        const Cand tau = cand[n - 1];
+        if (mine_best.s && !ahead(tau, mine_best))
+            for (int i = tid; i < total; i += MT) {
+                const Cand c = tile_cand(i);
+                if (c.s && !ahead(tau, c)) {
+                    const int at = atomicAdd(&n_picked, 1);            // at most n threads with BEAMS * TILES / MT = 32 tiles each
+                    picked[at] = c;
+                    picked_tile[at] = i;
+                }
+            }
+        __syncthreads();
+        p = n_picked;
+        for (int i = warp; i < p; i += MW) {
+            const int rank = rank_of(picked, p, i, lane);
+            if (lane == 0 && rank < n) chosen[rank] = i;
+        }
+        __syncthreads();
+        p = min(p, n);
+    } else if (tid < p) chosen[tid] = tid;
     __syncthreads();
-    for (int p = warp; p < n_picked; p += BT / 32) {
-        const int i = picked[p], b = i / slices;
-        if (lane < n) {
-            const u64 key = keys[((size_t)r * lists + i) * n + lane];
-            const double s = score(b, key);
-            const uint32_t at = place(b, key);
-            if (s > -INFINITY && !ahead(tau_s, tau_at, s, at)) {
-                const int slot = atomicAdd(&n_cand, 1);
-                cand_s[slot] = s;
-                cand_at[slot] = at;
+    // their candidates that are not below the bound
+    for (int t = warp; t < p; t += MW) {
+        const int i = picked_tile[chosen[t]];
+        const Tile tile = mine[i];
+        const int b = beam_of(tile), lo = (i - b * tiles) * TILE;
+        const Beam beam = beams[b];
+        // a logit below this has a score below the bound: a few roundings of 64 bits and the conversion are within 2^-20 of the sizes
+        const double at_least = (double)bound - beam.base + beam.lse;
+        const float least = beam.shares ? INFINITY : (float)(at_least - 1e-6 * (fabs(at_least) + fabs((double)bound) + fabs(beam.base) + fabs(beam.lse)));
+        if (tile.second < least || tile.second == -INFINITY) {         // usually: the tile's best is its only candidate
+            if (lane == 0) cand[atomicAdd(&n_cand, 1)] = picked[chosen[t]];
+            continue;
+        }
+        const float* const w = logits + (long long)(r * K + b) * ldl;
+        float v[PER];
+        load_tile<VEC>(v, w, lo, V, lane);
+        uint32_t in = 0;
+        #pragma unroll
+        for (int e = 0; e < PER; e++) in |= !(v[e] < least) && v[e] > -INFINITY ? 1u << e : 0u;
+        const int count = __reduce_add_sync(0xffffffffu, __popc(in));
+        int base = 0;
+        if (lane == 0) base = atomicAdd(&n_cand, min(count, n));
+        base = __shfl_sync(0xffffffffu, base, 0);
+        auto put = [&](int slot, int at) { cand[slot] = cand_of(beam, w[at], (uint32_t)b * (uint32_t)V + (uint32_t)at); };
+        if (count <= n) {
+            int before = __popc(in);
+            #pragma unroll
+            for (int o = 1; o < 32; o <<= 1) { const int x = __shfl_up_sync(0xffffffffu, before, o); if (lane >= o) before += x; }
+            base += before - __popc(in);
+            for (; in; in &= in - 1) put(base++, lo + place_in<VEC>(__ffs(in) - 1, lane));
+        } else {
+            for (int j = 0; j < n; j++) {                              // the largest logit that is left, the first of equals
+                float top = -INFINITY;
+                int from = -1;
+                #pragma unroll
+                for (int e = PER - 1; e >= 0; e--)
+                    if ((in >> e & 1) && v[e] >= top) { top = v[e]; from = e; }
+                const uint32_t key = from < 0 ? 0u : order_key(top), most = __reduce_max_sync(0xffffffffu, key);
+                const int at = key == most ? place_in<VEC>(from, lane) : TILE, first = __reduce_min_sync(0xffffffffu, at);
+                if (at == first) { put(base + j, lo + at); in &= ~(1u << from); }
             }
         }
     }
     __syncthreads();
     const int c = n_cand;
-    for (int i = tid; i < c; i += BT) {
-        const double s = cand_s[i];
-        const uint32_t at = cand_at[i];
-        int rank = 0;
-        for (int j = 0; j < c; j++) rank += ahead(cand_s[j], cand_at[j], s, at);
-        if (rank < n) {
-            out_s[r * n + rank] = (float)s;
-            out_b[r * n + rank] = (int)(at / (uint32_t)V);
-            out_v[r * n + rank] = (int)(at % (uint32_t)V);
-        }
+    for (int i = warp; i < c; i += MW) {
+        const int rank = rank_of(cand, c, i, lane);
+        if (lane == 0 && rank < n) chosen[rank] = i;
     }
-    for (int i = c + tid; i < n; i += BT) { out_s[r * n + i] = -INFINITY; out_b[r * n + i] = out_v[r * n + i] = -1; }
+    __syncthreads();
+    if (tid < n) {
+        const bool is = tid < c;
+        const Cand me = is ? cand[chosen[tid]] : none();
+        const int b = (int)(me.at / (uint32_t)V);
+        out_s[r * n + tid] = is ? (float)order_value(me.s) : -INFINITY;
+        out_b[r * n + tid] = is ? b : -1;
+        out_v[r * n + tid] = is ? (int)(me.at - (uint32_t)b * (uint32_t)V) : -1;
+    }
 }
-
-int slices_of(int V) { return (V + SLICE - 1) / SLICE; }
 
 }  // namespace
 
-// Bytes of scratch, or -1 where the sizes are not supported.
-IK_EXPORT long long ik_beam_select_scratch(int R, int K, int V, int n) {
-    if (R <= 0 || K <= 0 || V <= 0 || n <= 0 || K > BEAMS || n > OUT || slices_of(V) > SLICES || (long long)R * K > 0x7fffffff / 2) return -1;
-    return (long long)R * K * slices_of(V) * (n * 8ll + 16);
-}
-
-// scratch: ik_beam_select_scratch bytes on 16 bytes.
-IK_EXPORT int ik_beam_select(const float* logits, long long ldl, const float* sums, int R, int K, int V, int n, void* scratch, float* out_s,
+// scratch: 16 bytes for every 1,024 logits of a row, or part of them, on 16 bytes.  At most 16 beams, 32 results, 1,048,576 logits.
+IK_EXPORT int ik_beam_select(const float* logits, long long ldl, const float* sums, int R, int K, int V, int n, void* scratch, long long scratch_bytes, float* out_s,
                              int* out_b, int* out_v, cudaStream_t stream) {
-    if (ik_beam_select_scratch(R, K, V, n) < 0 || (ldl < V && R * K > 1) || ((uintptr_t)logits & 3) || ((uintptr_t)scratch & 15)) return IK_BAD_ARGUMENT;
-    const int slices = slices_of(V);
-    double2* const stats = reinterpret_cast<double2*>(scratch);
-    u64* const keys = reinterpret_cast<u64*>(stats + (size_t)R * K * slices);
-    IK_RETURN_IF_ERROR(ik_launch(beam_rows_kernel, dim3(R * K, slices), BT, 0, stream, logits, ldl, sums, V, n, slices, keys, stats));
-    const size_t smem = (size_t)K * slices * 12;
-    IK_RETURN_IF_ERROR(ik_launch(beam_merge_kernel, dim3(R), BT, smem, stream, (const u64*)keys, (const double2*)stats, sums, K, V, n, slices, out_s, out_b, out_v));
+    const int tiles = (V + TILE - 1) / TILE;
+    if (R <= 0 || K <= 0 || V <= 0 || n <= 0 || K > BEAMS || n > OUT || tiles > TILES || (long long)R * K > 0x3fffffff || scratch_bytes < (long long)R * K * tiles * 16 ||
+        (ldl < V && R * K > 1) || ((uintptr_t)logits & 3) || ((uintptr_t)scratch & 15))
+        return IK_BAD_ARGUMENT;
+    Tile* const t = reinterpret_cast<Tile*>(scratch);
+    const dim3 grid(R * K, (tiles + RT / 32 - 1) / (RT / 32));
+    const bool vec = V % 4 == 0 && ldl % 4 == 0 && ((uintptr_t)logits & 15) == 0;
+    IK_RETURN_IF_ERROR(vec ? ik_launch(beam_tiles_kernel<true>, grid, RT, 0, stream, logits, ldl, sums, K, V, tiles, t)
+                           : ik_launch(beam_tiles_kernel<false>, grid, RT, 0, stream, logits, ldl, sums, K, V, tiles, t));
+    IK_RETURN_IF_ERROR(vec ? ik_launch_family(IK_FAMILY_ELEMENTWISE, beam_merge_kernel<true>, dim3(R), MT, 0, stream, logits, ldl, (const Tile*)t, sums, K, V, n, tiles, out_s, out_b, out_v)
+                           : ik_launch_family(IK_FAMILY_ELEMENTWISE, beam_merge_kernel<false>, dim3(R), MT, 0, stream, logits, ldl, (const Tile*)t, sums, K, V, n, tiles, out_s, out_b, out_v));
     IK_LAUNCH_STATUS();
 }

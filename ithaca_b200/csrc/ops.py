@@ -1235,8 +1235,8 @@ def _search_lib():
     global _search
     if _search is None:
         l = build.search()
-        l.ik_beam_select_scratch.argtypes, l.ik_beam_select_scratch.restype = [_i, _i, _i, _i], ctypes.c_longlong
-        l.ik_beam_select.argtypes, l.ik_beam_select.restype = [_vp, ctypes.c_longlong, _vp, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp], _i
+        ll = ctypes.c_longlong
+        l.ik_beam_select.argtypes, l.ik_beam_select.restype = [_vp, ll, _vp, _i, _i, _i, _i, _vp, ll, _vp, _vp, _vp, _vp], _i
         l.ik_copy_rows.argtypes, l.ik_copy_rows.restype = [_vp, _i, _vp, _i, _vp], _i
         _search = l
     return timed(_search)
@@ -1276,14 +1276,11 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n_out: int, out: Opt
         _here(out, "out")
         if out.shape != (3, R, n_out):
             raise KernelError(f"beam_select: out must be [3, {R}, {n_out}], found {tuple(out.shape)}")
-    library = _search_lib()
-    need = library.ik_beam_select_scratch(R, K, V, n_out)
-    if need < 0:
-        raise KernelError("beam_select: these sizes are not supported")
+    need = R * K * -(-V // 1024) * 16
     scratch = torch.empty(need, dtype=torch.uint8, device=logits.device)
     s, b, v = out.unbind(0)
     _work(f"beam select {R}x{K}x{V}", R * K * V * 4 + need)
-    _check(library.ik_beam_select(_ptr(logits), logits.stride(0), _ptr(scores), R, K, V, n_out, _ptr(scratch), _ptr(s), _ptr(b), _ptr(v), _stream()),
+    _check(_search_lib().ik_beam_select(_ptr(logits), logits.stride(0), _ptr(scores), R, K, V, n_out, _ptr(scratch), need, _ptr(s), _ptr(b), _ptr(v), _stream()),
            "beam_select", kernels=2)
     return s.view(torch.float32), b, v
 
