@@ -228,21 +228,14 @@ def shared_module(head_dim: int) -> ctypes.CDLL:
     m = _shared_modules.get(head_dim)
     if m is None:
         m = build.load_library(*build.shared_module(head_dim))
-        m.ik_attn_shared.argtypes = [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp, _vp, _i, _i, _i, _i, _i, _f, _f, _i, _vp, _i, _i, _i, _i, _i, _i, _vp, _vp]
+        m.ik_attn_shared.argtypes = [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp, _vp, _i, _i, _i, _i, _i, _f, _f, _i, _vp, _i, _i, _vp, _vp]
         m.ik_attn_shared.restype = _i
+        m.ik_attn_shared_scratch.argtypes, m.ik_attn_shared_scratch.restype = [_i, _i, _i, _i, _i], ctypes.c_longlong
+        m.ik_attn_shared_take_wait_record.argtypes, m.ik_attn_shared_take_wait_record.restype = [_vp], _i
         if m.ik_attn_shared_head_dim() != head_dim:
             raise KernelError("the attention module was compiled for another head size")
         _shared_modules[head_dim] = m
     return ops.timed(m)
-
-
-def shared_chunks(n_groups: int, max_members: int, n_seqs: int, n_heads: int, n_kv_heads: int, hd: int, shared_bound: int, own_bound: int, n_sm: int) -> Tuple[int, int]:
-    """Pages per block of the shared and of the own pages."""
-    rows = 16 * (4 if hd <= 64 else 2 if hd <= 128 else 1)
-    per = n_heads // n_kv_heads
-    blocks = max(1, n_groups * n_kv_heads * -(-(max_members * per) // rows))
-    n_shared = max(1, 2 * n_sm // blocks)
-    return max(2, -(-max(1, shared_bound) // n_shared)), 4
 
 
 def sharing_pays(starts, pages, n_pages, n_kv_heads: int, hd: int) -> bool:
@@ -253,41 +246,37 @@ def sharing_pays(starts, pages, n_pages, n_kv_heads: int, hd: int) -> bool:
 def decode_shared(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, kv_lens: torch.Tensor, table: torch.Tensor, starts: torch.Tensor,
                   shared: torch.Tensor, n_groups: int, max_members: int, shared_bound: int, own_bound: int, n_heads: int, scale: float,
                   status: Optional[torch.Tensor], out: Optional[torch.Tensor] = None, softcap: float = 0.0, sink=False,
-                  chunks: Optional[Tuple[int, int]] = None, work: Optional[Tuple[int, int]] = None) -> torch.Tensor:
+                  work: Optional[Tuple[int, int]] = None) -> torch.Tensor:
     """Attention of one new token per sequence (``q`` [B, heads * size], bfloat16) over pages of which groups of sequences share the first ones.  ``starts`` int32
     [n_groups + 1]: group g are the sequences starts[g] <= b < starts[g + 1], at most ``max_members`` of them; ``shared`` int32 [B]: how many of sequence b's first pages are
-    the same (and full) in all of its group, 0 for a sequence that shares none.  ``shared_bound``, ``own_bound``: about how many pages a group shares and a
-    sequence has of its own at most; they size the grid and the scratch, and a bound that is too small costs time, not the result.  All else as
-    ``decode`` has it, without a window."""
+    the same (and full) in all of its group, 0 for a sequence that shares none; a sequence that is in no group gets zeros.  ``shared_bound``, ``own_bound``: about how many pages a group
+    shares and a sequence has of its own at most (the kernel sees the numbers themselves; they are for the caller's choice between this and ``decode``).  At most 1,024 sequences.  All else
+    as ``decode`` has it, without a window."""
     n_pages, nkv, page_size, hd = k_pages.shape
-    B = kv_lens.shape[0]
-    if q.dtype != torch.bfloat16 or k_pages.dtype != torch.bfloat16 or v_pages.dtype != torch.bfloat16:
-        raise KernelError("decode_shared: queries and pages must be bfloat16")
+    B, bf16, i32 = kv_lens.shape[0], torch.bfloat16, torch.int32
     if not supported(hd) or page_size != 64 or v_pages.shape != k_pages.shape:
         raise KernelError("decode_shared: pages of 64 keys and values of one head size, a multiple of 16 up to 256, are supported")
     if n_heads % nkv or q.numel() != B * n_heads * hd:
         raise KernelError(f"decode_shared: queries {tuple(q.shape)} are not {B} times {n_heads} heads of {hd} on {nkv} kv heads")
-    for t, name in ((q, "q"), (k_pages, "k_pages"), (v_pages, "v_pages")):
-        ops._need(t, name)
+    for t, name, dtype in ((q, "q", bf16), (k_pages, "k_pages", bf16), (v_pages, "v_pages", bf16), (kv_lens, "kv_lens", i32), (starts, "starts", i32), (shared, "shared", i32)):
+        ops._need(t, name, dtype)
         ops._here(t, name)
-    for t, name, n in ((kv_lens, "kv_lens", B), (starts, "starts", n_groups + 1), (shared, "shared", B)):
-        ops._need(t, name, torch.int32)
-        if t.numel() != n:
-            raise KernelError(f"decode_shared: {name} has {t.numel()} elements, {n} are needed")
-    ops._need(table, "table", torch.int32, contiguous=False)
-    if table.dim() != 2 or table.shape[0] != B or table.stride(1) != 1 or n_groups < 0 or not 1 <= max_members <= B:
+    ops._need(table, "table", i32, contiguous=False)
+    if starts.numel() != n_groups + 1 or shared.numel() != B:
+        raise KernelError(f"decode_shared: {n_groups + 1} starts and {B} numbers of shared pages are needed, found {starts.numel()} and {shared.numel()}")
+    if table.dim() != 2 or table.shape[0] != B or table.stride(1) != 1 or n_groups < 1 or not 1 <= max_members <= B:
         raise KernelError("decode_shared: the block table is [sequences, pages], and a group has between one and all of the sequences")
     m = shared_module(hd)
-    c_shared, c_own = chunks or shared_chunks(n_groups, max_members, B, n_heads, nkv, hd, shared_bound, own_bound, sm_count())
-    n_shared, n_own = max(1, -(-shared_bound // c_shared)), max(1, -(-own_bound // c_own))
-    part_o = torch.empty((B, n_heads, n_shared + n_own, hd + 2), dtype=torch.float32, device=q.device)
-    part_ml = _ptr(part_o) + B * n_heads * (n_shared + n_own) * hd * 4
+    need = m.ik_attn_shared_scratch(n_groups, max_members, B, n_heads, nkv)
+    if need < 0:
+        raise KernelError(f"decode_shared: {B} sequences in {n_groups} groups of up to {max_members} are more than this kernel takes")
+    scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
     if out is None:
         out = torch.empty_like(q)
     ops._work(f"attention decode shared {B}x{n_heads}", *(work or (0, 0)))
-    _check(m.ik_attn_shared(_ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(out), _ptr(part_o), part_ml, _ptr(kv_lens), _ptr(table), table.stride(0), table.shape[1],
-                            _ptr(starts), _ptr(shared), n_groups, max_members, B, n_heads, nkv, scale, softcap, ops.sink_flag(sink), _ptr(ops.sink_values(sink, n_heads)),
-                            page_size, n_pages, c_shared, n_shared, c_own, n_own, _ptr(status), _stream()), "attention decode (shared pages)", kernels=2)
+    _check(m.ik_attn_shared(_ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(out), _ptr(scratch), _ptr(kv_lens), _ptr(table), table.stride(0), table.shape[1], _ptr(starts),
+                            _ptr(shared), n_groups, max_members, B, n_heads, nkv, scale, softcap, ops.sink_flag(sink), _ptr(ops.sink_values(sink, n_heads)), page_size, n_pages,
+                            _ptr(status), _stream()), "attention decode (shared pages)", kernels=2)
     return out
 
 

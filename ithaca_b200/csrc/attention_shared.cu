@@ -1,17 +1,26 @@
 // Attention of one new token per sequence where groups of sequences share their first pages, specialised at compile time for one head size
 // (IK_HD, a multiple of 16).  bfloat16 pages of 64 keys, as attention_bf16.cu has them.
 //
-// o[i,h] = sum_j p_j v[j] with p = softmax_j(q[i,h] . k[j] scale) over the keys of sequence i, head h reading kv head h / (nh / nkv).  Sequences starts[g] <= i <
-// starts[g+1] form group g, whose first shared[i] pages are the same: what they contribute is formed once for the group, with the rows (sequence, query
-// head of the kv head) of all members as the rows of one tile, so that a shared key or value is read once for all of them; the pages behind are
-// each sequence's own.  A block owns a tile of rows, a kv head and one chunk of pages and leaves an unnormalised partial (maximum,
-// sum, output) per row; a second kernel joins a row's partials in the order of its chunks.
+// o[i,h] = sum_j p_j v[j] with p = softmax_j(q[i,h] . k[j] scale) over the keys j of sequence i, head h reading kv head h / G, G = nh / nkv.  Sequences
+// starts[g] <= i < starts[g+1] form group g, whose first shared[i] pages are the same.  A tile is some of a group's members with their G heads of a kv head: ROWS rows
+// at most (heads in parts where G is more than that).  It sees a list of pages: the shared ones, which count for all of its rows, then every member's own,
+// which count for that member's rows.  So a shared page is read once for all members of a tile, as the keys and values of one product.
 //
-// Keys behind a sequence's length are masked by position.  A page index outside the pool sets *status and is not followed.  A sequence
-// without keys gets zeros.
+// The pages of all tiles, one list behind the other, are cut into equal runs, a block each (per kv head): every block streams as many pages as every other,
+// however unequal the groups are.  Where a run passes from one tile to the next, the block leaves the first one's partial result (unnormalised output,
+// maximum, sum) and goes on; a second kernel joins each row's partials in the order of their runs.  Run j's partial of tile t is kept at t + j: each new
+// partial is one tile or one run further, so the numbers are distinct and dense.
+//
+// A block: one warp brings pages into a ring of shared memory (cp.async), four compute on mma.sync m16n8k16 tiles.  A warp owns 16 rows and 64 / KQ
+// of a page's keys (RT = 1, 2 or 4 tiles of 16 rows, KQ = 4 / RT), with running maximum and sum as floats, base 2; the warps of equal rows are merged at the
+// end of a tile.  Probabilities are rounded to bfloat16 for the second product, as the other attention kernels do.
+//
+// Keys behind a sequence's length are masked by position and their values are brought as zeros, so what lies in the unused part of a page never
+// matters.  A page index outside the pool sets *status and is not followed.  A sequence without keys gets zeros.
 #include <math.h>
 #define IK_FAMILY 4
 #include "common.cuh"
+#include "tc_common.cuh"
 
 #ifndef IK_HD
 #error "compile with -DIK_HD=<head size>"
@@ -22,28 +31,30 @@ namespace {
 constexpr int HD = IK_HD;
 constexpr int PAGE = 64;
 constexpr int LD = HD + 8;                 // padded row: consecutive rows fall into different banks
-constexpr int MT = HD <= 64 ? 4 : HD <= 128 ? 2 : 1;     // tiles of 16 rows a block: what the registers hold of their outputs
-constexpr int ROWS = 16 * MT;
+constexpr int STAGE = 2 * PAGE * LD;       // keys and values of a page, in elements
+constexpr int NS = HD <= 64 ? 4 : 3;       // pages of the ring: 104 KB at head size 128, two blocks to an SM
+constexpr int BLOCKS = HD <= 128 ? 2 : 1;  // blocks of an SM
+constexpr int THREADS = 160;               // four computing warps, one that loads
+constexpr int TILES = 1024, SEQS = 1024;   // most tiles and sequences of a launch
+constexpr int LEAST = 2;                   // least pages of a run: a block's set-up and its partial cost about as much as two
 static_assert(HD % 16 == 0 && HD >= 16 && HD <= 256, "head size must be a multiple of 16 up to 256");
 
 typedef __nv_bfloat16 bf16;
 
-__device__ __forceinline__ void cp16(void* smem, const void* gmem, bool valid) {
-    const uint32_t s = (uint32_t)__cvta_generic_to_shared(smem);
+__device__ __forceinline__ void cp16(uint32_t smem, const void* gmem, bool valid) {
     const int n = valid ? 16 : 0;
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" :: "r"(s), "l"(gmem), "r"(n));
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" :: "r"(smem), "l"(gmem), "r"(n));
 }
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;\n"); }
-template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;\n" :: "n"(N)); }
-__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], const void* p) {
-    const uint32_t s = (uint32_t)__cvta_generic_to_shared(p);
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(s));
+// Arrives on the barrier when this thread's copies so far have landed.
+__device__ __forceinline__ void cp_arrive(uint64_t* bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" :: "r"(smem_u32(bar)) : "memory");
 }
-__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], const void* p) {
-    const uint32_t s = (uint32_t)__cvta_generic_to_shared(p);
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(s));
+__device__ __forceinline__ void compute_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t s) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(s) : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t s) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(s) : "memory");
 }
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
@@ -63,283 +74,416 @@ __device__ __forceinline__ float capped(float s, float a, float b) {
     return b * y;
 }
 
-// How the work is cut: shared pages into at most n_shared chunks of shared_chunk pages, own pages into at most n_own of own_chunk; the last
-// chunk of a kind takes all that is left, so that a bound that was too small costs time and nothing else.
-struct Cut { int shared_chunk, n_shared, own_chunk, n_own; };
-__device__ __forceinline__ int chunks_of(int pages, int chunk, int most) { return min(most, (pages + chunk - 1) / chunk); }
+// What both kernels get.  Tile number: (group, part of its members, part of the heads), tiles_per_group to each group whether it has so many members or not.
+struct Call {
+    const int *kv_lens, *table, *starts, *shared;
+    int table_stride, table_cols, n_groups, B, nh, nkv, G;
+    int members, heads, head_parts, tiles_per_group, n_tiles;       // members and heads of a tile; parts of the heads; tiles
+    int runs;
+};
+struct TileOf { int first, last, part, S; };                          // members first <= i < last, part of the heads, pages they share
+__device__ __forceinline__ TileOf tile_of(const Call& c, int t) {
+    const int g = t / c.tiles_per_group, k = t % c.tiles_per_group;
+    const int a = min(max(c.starts[g], 0), c.B), b = min(max(c.starts[g + 1], a), c.B);
+    TileOf o;
+    o.part = k % c.head_parts;
+    o.first = min(a + k / c.head_parts * c.members, b);
+    o.last = min(o.first + c.members, b);
+    o.S = a < b ? min(max(c.shared[a], 0), c.table_cols) : 0;
+    return o;
+}
+// pages: how many every sequence has, shared ones included.
+__device__ __forceinline__ int own_pages(const int* pages, const TileOf& o, int seq) { return max(0, pages[seq] - o.S); }
+__device__ __forceinline__ int pages_in(const int* pages, const TileOf& o) {
+    if (o.first >= o.last) return 0;
+    int n = o.S;
+    for (int i = o.first; i < o.last; i++) n += own_pages(pages, o, i);
+    return n;
+}
+// Runs in use, the first page of a run, the run of a page.
+__device__ __forceinline__ int runs_of(int pages, int runs) { return min(runs, (pages + LEAST - 1) / LEAST); }
+__device__ __forceinline__ int run_start(int j, int pages, int runs) { return (int)((long long)j * pages / runs); }
+__device__ __forceinline__ int run_of(int page, int pages, int runs) { return (int)((((long long)page + 1) * runs - 1) / pages); }
 
-// Rows of a block: (sequence, head) pairs; row r is head `first_head + r % heads` of sequence `first_seq + r / heads`.
-template <int NS>
-__global__ void __launch_bounds__(128)
+// The plan that the first block leaves for the join: per sequence its first tile and row, per tile its first and last run (no run: 1, 0).
+struct Plan { int2* seqs; int2* tiles; };
+
+template <int RT>
+__global__ void __launch_bounds__(THREADS, BLOCKS)
 attn_shared_kernel(const bf16* __restrict__ q, const bf16* __restrict__ k_pages, const bf16* __restrict__ v_pages, float* __restrict__ part_o,
-                   float* __restrict__ part_ml, const int* __restrict__ kv_lens, const int* __restrict__ table, int table_stride, int table_cols,
-                   const int* __restrict__ starts, const int* __restrict__ shared, int n_groups, int row_tiles, int B, int nh, int nkv, float scale_log2e,
-                   float cap_log2e, int n_pages, Cut cut, int* status) {
+                   float2* __restrict__ part_ml, const Call c, const Plan plan, float scale_log2e, float cap_log2e, int n_pages, int* status) {
+    constexpr int ROWS = 16 * RT, KQ = 4 / RT, KEYS = PAGE / KQ, NB = KEYS / 8, CH = HD / 8;
     ik_pdl_wait();
-    constexpr int CH = HD / 8;
     extern __shared__ __align__(16) unsigned char smem_raw[];
-    bf16* Qs = (bf16*)smem_raw;                      // [ROWS][LD]
-    bf16* Ks = Qs + ROWS * LD;                       // [NS][PAGE][LD]
-    bf16* Vs = Ks + NS * PAGE * LD;                  // [NS][PAGE][LD]
-    __shared__ int row_pos[ROWS];                    // the query's position, -1: no such row
+    bf16* const ring = (bf16*)smem_raw;                              // [NS][keys, values][PAGE][LD]
+    int* const ends = (int*)(smem_raw + (size_t)NS * STAGE * sizeof(bf16));     // [n_tiles]: pages up to and with a tile
+    int* const pages = ends + c.n_tiles;                             // [B]
+    __shared__ uint64_t full[NS], empty[NS];
+    __shared__ int abort_flag;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, run = blockIdx.x, kvh = blockIdx.y;
 
-    const int kvh = blockIdx.y, G = nh / nkv;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int shared_blocks = n_groups * row_tiles * cut.n_shared;
-    int first_seq, n_rows, first_row, p_first, p_end, split;      // rows first_row .. of the (sequence, head) pairs from first_seq on
-    int filled = 0x7fffffff;                                       // positions of own pages that hold keys (shared pages are full)
-    if ((int)blockIdx.x < shared_blocks) {
-        int i = blockIdx.x;
-        split = i % cut.n_shared; i /= cut.n_shared;
-        const int rt = i % row_tiles, grp = i / row_tiles;
-        first_seq = min(max(starts[grp], 0), B);
-        const int members = min(max(starts[grp + 1], first_seq), B) - first_seq;
-        first_row = rt * ROWS;
-        n_rows = min(ROWS, members * G - first_row);
-        if (n_rows <= 0) return;
-        const int pages = min(max(shared[first_seq], 0), table_cols), n = chunks_of(pages, cut.shared_chunk, cut.n_shared);
-        if (split >= n) return;
-        p_first = split * cut.shared_chunk;
-        p_end = split == n - 1 ? pages : p_first + cut.shared_chunk;
-    } else {
-        const int hc_n = (G + ROWS - 1) / ROWS;
-        int i = blockIdx.x - shared_blocks;
-        const int os = i % cut.n_own; i /= cut.n_own;
-        first_seq = i / hc_n;
-        first_row = (i % hc_n) * ROWS;
-        n_rows = min(ROWS, G - first_row);
-        filled = kv_lens[first_seq];
-        const int pages = min((max(filled, 0) + PAGE - 1) / PAGE, table_cols), mine = min(max(shared[first_seq], 0), pages);
-        const int n = chunks_of(pages - mine, cut.own_chunk, cut.n_own);
-        if (os >= n) return;
-        p_first = mine + os * cut.own_chunk;
-        p_end = os == n - 1 ? pages : p_first + cut.own_chunk;
-        split = cut.n_shared + os;
+    if (tid == 0) {
+        abort_flag = 0;
+        #pragma unroll
+        for (int s = 0; s < NS; s++) { mbar_init(&full[s], 32); mbar_init(&empty[s], 4); }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    const int n_mt = (n_rows + 15) / 16;
-    const int* const pages_of = table + (size_t)first_seq * table_stride;
-    for (int r = threadIdx.x; r < ROWS; r += 128) row_pos[r] = r < n_rows ? kv_lens[first_seq + (first_row + r) / G] - 1 : -1;
-    for (int idx = threadIdx.x; idx < n_mt * 16 * CH; idx += 128) {
-        const int r = idx / CH, c = idx % CH, rho = first_row + r;
-        const bool v = r < n_rows;
-        cp16(Qs + r * LD + c * 8, v ? q + ((size_t)(first_seq + rho / G) * nh + kvh * G + rho % G) * HD + c * 8 : q, v);
-    }
-    auto load_page = [&](int stage, int p) {
-        int page = pages_of[p];
-        if (page < 0 || page >= n_pages) { if (threadIdx.x == 0) ik_set_status(status, IK_STATUS_READ_NO_PAGE); page = 0; }
-        const bf16* kg = k_pages + ((size_t)page * nkv + kvh) * PAGE * HD;
-        const bf16* vg = v_pages + ((size_t)page * nkv + kvh) * PAGE * HD;
-        bf16* ks = Ks + stage * PAGE * LD;
-        bf16* vs = Vs + stage * PAGE * LD;
-        for (int idx = threadIdx.x; idx < PAGE * CH; idx += 128) {
-            const int r = idx / CH, c = idx % CH;
-            cp16(ks + r * LD + c * 8, kg + r * HD + c * 8, true);
-            cp16(vs + r * LD + c * 8, vg + r * HD + c * 8, p * PAGE + r < filled);      // what lies behind the last key has weight 0 and may be anything: not even 0 x NaN
+    for (int i = tid; i < c.B; i += THREADS) pages[i] = min((max(c.kv_lens[i], 0) + PAGE - 1) / PAGE, c.table_cols);
+    __syncthreads();
+    for (int t = tid; t < c.n_tiles; t += THREADS) ends[t] = pages_in(pages, tile_of(c, t));
+    __syncthreads();
+    if (warp == 0) {
+        int before = 0;
+        for (int t0 = 0; t0 < c.n_tiles; t0 += 32) {
+            int x = t0 + lane < c.n_tiles ? ends[t0 + lane] : 0;
+            #pragma unroll
+            for (int o = 1; o < 32; o <<= 1) { const int y = __shfl_up_sync(0xffffffffu, x, o); if (lane >= o) x += y; }
+            if (t0 + lane < c.n_tiles) ends[t0 + lane] = before + x;
+            before += __shfl_sync(0xffffffffu, x, 31);
         }
-    };
-    #pragma unroll
-    for (int s = 0; s < NS; s++) {
-        if (p_first + s < p_end) load_page(s, p_first + s);
-        cp_commit();
+    }
+    __syncthreads();
+    const int total = ends[c.n_tiles - 1], runs = total > 0 ? runs_of(total, c.runs) : 0;
+    if (run == 0 && kvh == 0) {
+        for (int i = tid; i < c.B; i += THREADS) plan.seqs[i] = make_int2(-1, 0);
+        __syncthreads();
+        for (int t = tid; t < c.n_tiles; t += THREADS) {
+            const int lo = t ? ends[t - 1] : 0, hi = ends[t];
+            plan.tiles[t] = lo < hi ? make_int2(run_of(lo, total, runs), run_of(hi - 1, total, runs)) : make_int2(1, 0);
+            const TileOf o = tile_of(c, t);
+            if (o.part == 0)
+                for (int i = o.first; i < o.last; i++) plan.seqs[i] = make_int2(t, (i - o.first) * c.heads);
+        }
+    }
+    if (run >= runs) return;
+    const int u_first = run_start(run, total, runs), u_end = run_start(run + 1, total, runs);
+    int t = 0;
+    while (ends[t] <= u_first) t++;
+
+    if (warp == 4) {
+        // ---- the loader: 32 pages' numbers at a time, one each lane
+        int step = 0;
+        bool alive = true;
+        for (int u = u_first; u < u_end && alive;) {
+            while (ends[t] <= u) t++;
+            const int lo = t ? ends[t - 1] : 0, n = min(min(ends[t], u_end) - u, 32);
+            const TileOf o = tile_of(c, t);
+            int page = 0, filled = PAGE;
+            if (lane < n) {
+                int i = u + lane - lo, seq = o.first, col = i;
+                if (i >= o.S) {
+                    i -= o.S;
+                    for (int own = own_pages(pages, o, seq); i >= own; own = own_pages(pages, o, seq)) { i -= own; seq++; }
+                    col = o.S + i;
+                    filled = c.kv_lens[seq] - col * PAGE;
+                }
+                page = c.table[(size_t)seq * c.table_stride + col];
+                if (page < 0 || page >= n_pages) { ik_set_status(status, IK_STATUS_READ_NO_PAGE); page = 0; }
+            }
+            for (int l = 0; l < n; l++, step++) {
+                const int stage = step % NS, pg = __shfl_sync(0xffffffffu, page, l), rows = __shfl_sync(0xffffffffu, filled, l);
+                alive = __all_sync(0xffffffffu, step < NS || mbar_wait(&empty[stage], (step / NS - 1) & 1, &abort_flag, status, IK_WAIT_LIMIT_NS, 41, step));
+                if (!alive) break;
+                const bf16* const kg = k_pages + ((size_t)pg * c.nkv + kvh) * PAGE * HD;
+                const bf16* const vg = v_pages + ((size_t)pg * c.nkv + kvh) * PAGE * HD;
+                const uint32_t to = smem_u32(ring + stage * STAGE);
+                #pragma unroll 8
+                for (int idx = lane; idx < PAGE * CH; idx += 32) cp16(to + (idx / CH * LD + idx % CH * 8) * 2, kg + idx * 8, true);
+                #pragma unroll 8
+                for (int idx = lane; idx < PAGE * CH; idx += 32) cp16(to + (PAGE * LD + idx / CH * LD + idx % CH * 8) * 2, vg + idx * 8, idx / CH < rows);
+                cp_arrive(&full[stage]);
+            }
+            u += n;
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        return;
     }
 
-    float o[MT][HD / 8][4], m_i[MT][2], l_i[MT][2];
-    #pragma unroll
-    for (int m = 0; m < MT; m++) {
+    // ---- the computing warps
+    const int g = lane >> 2, q2 = lane & 3, rt = warp % RT, kq = warp / RT;
+    int step = 0;
+    for (int u = u_first; u < u_end;) {
+        while (ends[t] <= u) t++;
+        const int lo = t ? ends[t - 1] : 0, stop = min(ends[t], u_end);
+        const TileOf o = tile_of(c, t);
+        const int n_rows = (o.last - o.first) * c.heads;             // rows of this tile (fewer where the last part of the heads is not full)
+        int seq_of[2], pos[2];
+        const bf16* qrow[2];
+        #pragma unroll
+        for (int r = 0; r < 2; r++) {
+            const int rho = rt * 16 + g + 8 * r, head = o.part * c.heads + rho % c.heads;
+            const bool is = rho < n_rows && head < c.G;
+            seq_of[r] = is ? o.first + rho / c.heads : -1;
+            pos[r] = is ? c.kv_lens[seq_of[r]] - 1 : -1;
+            qrow[r] = is ? q + ((size_t)seq_of[r] * c.nh + kvh * c.G + head) * HD + 2 * q2 : nullptr;
+        }
+        uint32_t qf[HD / 16][4];
+        #pragma unroll
+        for (int ks = 0; ks < HD / 16; ks++)
+            #pragma unroll
+            for (int e = 0; e < 4; e++) qf[ks][e] = qrow[e & 1] ? *reinterpret_cast<const uint32_t*>(qrow[e & 1] + ks * 16 + (e >> 1) * 8) : 0u;
+        // rows of a sequence that ends inside the shared pages, against what was asked for, are masked there, too
+        const bool ends_early = __any_sync(0xffffffffu, (seq_of[0] >= 0 && pos[0] + 1 < o.S * PAGE) || (seq_of[1] >= 0 && pos[1] + 1 < o.S * PAGE));
+        // which own page comes first
+        int member = o.first, col = u - lo;
+        if (col >= o.S) {
+            int i = col - o.S;
+            for (int own = own_pages(pages, o, member); i >= own; own = own_pages(pages, o, member)) { i -= own; member++; }
+            col = o.S + i;
+        }
+        float acc[HD / 8][4], m_i[2] = {-INFINITY, -INFINITY}, l_i[2] = {0.f, 0.f};
         #pragma unroll
         for (int d = 0; d < HD / 8; d++)
             #pragma unroll
-            for (int e = 0; e < 4; e++) o[m][d][e] = 0.f;
-        m_i[m][0] = m_i[m][1] = -INFINITY;
-        l_i[m][0] = l_i[m][1] = 0.f;
-    }
+            for (int e = 0; e < 4; e++) acc[d][e] = 0.f;
 
-    for (int p = p_first; p < p_end; p++) {
-        const int stage = (p - p_first) % NS;
-        cp_wait<NS - 1>();
-        __syncthreads();
-        const bf16* ks_ = Ks + (stage * PAGE + warp * 16) * LD;
-        const bf16* vs_ = Vs + (stage * PAGE + warp * 16) * LD;
-        float s[MT][2][4];
-        #pragma unroll
-        for (int m = 0; m < MT; m++)
-            #pragma unroll
-            for (int n = 0; n < 2; n++)
-                #pragma unroll
-                for (int e = 0; e < 4; e++) s[m][n][e] = 0.f;
-        #pragma unroll
-        for (int ks = 0; ks < HD / 16; ks++) {
-            uint32_t bfr[4];
-            ldsm4(bfr, ks_ + ((lane & 7) + (lane >> 4) * 8) * LD + ks * 16 + ((lane >> 3) & 1) * 8);
-            #pragma unroll
-            for (int m = 0; m < MT; m++)
-                if (m < n_mt) {
-                    uint32_t qf[4];
-                    ldsm4(qf, Qs + (m * 16 + (lane & 7) + ((lane >> 3) & 1) * 8) * LD + ks * 16 + (lane >> 4) * 8);
-                    mma(s[m][0], qf, bfr[0], bfr[1]);
-                    mma(s[m][1], qf, bfr[2], bfr[3]);
-                }
-        }
-        const int jbase = p * PAGE + warp * 16 + 2 * t;
-        uint32_t pa[MT][4];
-        #pragma unroll
-        for (int m = 0; m < MT; m++)
-            if (m < n_mt) {
-                const int pos[2] = {row_pos[m * 16 + g], row_pos[m * 16 + g + 8]};
-                float mx[2] = {-INFINITY, -INFINITY}, alpha[2], rs[2] = {0.f, 0.f};
-                #pragma unroll
-                for (int n = 0; n < 2; n++)
-                    #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const int r = e >> 1, j = jbase + n * 8 + (e & 1);
-                        const float v = j <= pos[r] ? capped(s[m][n][e], scale_log2e, cap_log2e) : -INFINITY;
-                        s[m][n][e] = v;
-                        mx[r] = fmaxf(mx[r], v);
-                    }
-                #pragma unroll
-                for (int r = 0; r < 2; r++) {
-                    mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
-                    mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
-                    const float m_new = fmaxf(m_i[m][r], mx[r]);
-                    const float m_use = m_new == -INFINITY ? 0.f : m_new;
-                    alpha[r] = exp2f(m_i[m][r] - m_use);
-                    m_i[m][r] = m_new;
-                    mx[r] = m_use;
-                }
-                #pragma unroll
-                for (int n = 0; n < 2; n++)
-                    #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const float pv = exp2f(s[m][n][e] - mx[e >> 1]);
-                        s[m][n][e] = pv;
-                        rs[e >> 1] += pv;
-                    }
-                #pragma unroll
-                for (int r = 0; r < 2; r++) l_i[m][r] = l_i[m][r] * alpha[r] + rs[r];
-                #pragma unroll
-                for (int d = 0; d < HD / 8; d++) {
-                    o[m][d][0] *= alpha[0]; o[m][d][1] *= alpha[0]; o[m][d][2] *= alpha[1]; o[m][d][3] *= alpha[1];
-                }
-                pa[m][0] = pack_bf16(s[m][0][0], s[m][0][1]);
-                pa[m][1] = pack_bf16(s[m][0][2], s[m][0][3]);
-                pa[m][2] = pack_bf16(s[m][1][0], s[m][1][1]);
-                pa[m][3] = pack_bf16(s[m][1][2], s[m][1][3]);
+        for (; u < stop; u++, step++) {
+            const bool own = u - lo >= o.S;
+            if (own && (u - lo == o.S || col >= pages[member])) {            // the next member that has pages of its own
+                if (u - lo != o.S) member++;
+                while (own_pages(pages, o, member) == 0) member++;
+                col = o.S;
             }
-        #pragma unroll
-        for (int dp = 0; dp < HD / 16; dp++) {
-            uint32_t bfr[4];
-            ldsm4t(bfr, vs_ + ((lane & 7) + ((lane >> 3) & 1) * 8) * LD + dp * 16 + (lane >> 4) * 8);
+            const int stage = step % NS;
+            if (!__all_sync(0xffffffffu, mbar_wait(&full[stage], (step / NS) & 1, &abort_flag, status, IK_WAIT_LIMIT_NS, 42, step))) return;
+            const uint32_t ks_ = smem_u32(ring + stage * STAGE + kq * KEYS * LD), vs_ = ks_ + PAGE * LD * 2;
+            float s[NB][4];
             #pragma unroll
-            for (int m = 0; m < MT; m++)
-                if (m < n_mt) {
-                    mma(o[m][2 * dp], pa[m], bfr[0], bfr[1]);
-                    mma(o[m][2 * dp + 1], pa[m], bfr[2], bfr[3]);
+            for (int n = 0; n < NB; n++)
+                #pragma unroll
+                for (int e = 0; e < 4; e++) s[n][e] = 0.f;
+            #pragma unroll
+            for (int ks = 0; ks < HD / 16; ks++)
+                #pragma unroll
+                for (int np = 0; np < NB / 2; np++) {
+                    uint32_t bfr[4];
+                    ldsm4(bfr, ks_ + (((np * 16 + (lane & 7) + (lane >> 4) * 8) * LD + ks * 16 + ((lane >> 3) & 1) * 8) * 2));
+                    mma(s[2 * np], qf[ks], bfr[0], bfr[1]);
+                    mma(s[2 * np + 1], qf[ks], bfr[2], bfr[3]);
                 }
-        }
-        __syncthreads();                                            // everyone is done with this stage
-        if (p + NS < p_end) load_page(stage, p + NS);
-        cp_commit();
-    }
-    cp_wait<0>();
-    ik_pdl_launch_dependents();
-    // the four warps' partial results, merged in warp order (the ring is free now)
-    float* sm_o = (float*)Ks;                         // [4][ROWS][HD]
-    float* sm_ml = sm_o + 4 * ROWS * HD;              // [4][ROWS][2]
-    #pragma unroll
-    for (int m = 0; m < MT; m++)
-        if (m < n_mt) {
+            float mx[2] = {-INFINITY, -INFINITY};
+            if (own || ends_early) {
+                const int jbase = (own ? col : u - lo) * PAGE + kq * KEYS + 2 * q2;
+                #pragma unroll
+                for (int n = 0; n < NB; n++)
+                    #pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int r = e >> 1;
+                        const bool ok = (!own || seq_of[r] == member) && jbase + n * 8 + (e & 1) <= pos[r];
+                        s[n][e] = ok ? capped(s[n][e], scale_log2e, cap_log2e) : -INFINITY;
+                        mx[r] = fmaxf(mx[r], s[n][e]);
+                    }
+            } else {
+                #pragma unroll
+                for (int n = 0; n < NB; n++)
+                    #pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        s[n][e] = capped(s[n][e], scale_log2e, cap_log2e);
+                        mx[e >> 1] = fmaxf(mx[e >> 1], s[n][e]);
+                    }
+            }
+            col += own;
+            float alpha[2], rs[2] = {0.f, 0.f};
             #pragma unroll
             for (int r = 0; r < 2; r++) {
-                float l = l_i[m][r];
-                l += __shfl_xor_sync(0xffffffffu, l, 1);
-                l += __shfl_xor_sync(0xffffffffu, l, 2);
-                const int row = warp * ROWS + m * 16 + g + 8 * r;
-                #pragma unroll
-                for (int d = 0; d < HD / 8; d++) {
-                    sm_o[row * HD + d * 8 + 2 * t] = o[m][d][2 * r];
-                    sm_o[row * HD + d * 8 + 2 * t + 1] = o[m][d][2 * r + 1];
-                }
-                if (t == 0) { sm_ml[row * 2] = m_i[m][r]; sm_ml[row * 2 + 1] = l; }
+                mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
+                mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
+                const float m_new = fmaxf(m_i[r], mx[r]), m_use = m_new == -INFINITY ? 0.f : m_new;
+                alpha[r] = ik_ex2(m_i[r] - m_use);
+                m_i[r] = m_new;
+                mx[r] = m_use;
             }
+            uint32_t pa[NB / 2][4];
+            #pragma unroll
+            for (int n = 0; n < NB; n++) {
+                #pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    s[n][e] = ik_ex2(s[n][e] - mx[e >> 1]);
+                    rs[e >> 1] += s[n][e];
+                }
+                pa[n / 2][(n & 1) * 2] = pack_bf16(s[n][0], s[n][1]);
+                pa[n / 2][(n & 1) * 2 + 1] = pack_bf16(s[n][2], s[n][3]);
+            }
+            #pragma unroll
+            for (int r = 0; r < 2; r++) l_i[r] = l_i[r] * alpha[r] + rs[r];
+            if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+                #pragma unroll
+                for (int d = 0; d < HD / 8; d++) { acc[d][0] *= alpha[0]; acc[d][1] *= alpha[0]; acc[d][2] *= alpha[1]; acc[d][3] *= alpha[1]; }
+            }
+            #pragma unroll
+            for (int kk = 0; kk < NB / 2; kk++)
+                #pragma unroll
+                for (int dp = 0; dp < HD / 16; dp++) {
+                    uint32_t bfr[4];
+                    ldsm4t(bfr, vs_ + (((kk * 16 + (lane & 7) + ((lane >> 3) & 1) * 8) * LD + dp * 16 + (lane >> 4) * 8) * 2));
+                    mma(acc[2 * dp], pa[kk], bfr[0], bfr[1]);
+                    mma(acc[2 * dp + 1], pa[kk], bfr[2], bfr[3]);
+                }
+            __syncwarp();
+            // the last page of a tile is given back behind the merge below, which uses its space
+            if (lane == 0 && (KQ == 1 || u + 1 < stop)) mbar_arrive(&empty[stage]);
         }
-    __syncthreads();
-    const int n_splits = cut.n_shared + cut.n_own;
-    for (int idx = threadIdx.x; idx < n_rows * HD; idx += 128) {
-        const int r = idx / HD, x = idx % HD, rho = first_row + r;
-        float mm = -INFINITY;
+        const size_t slot = (size_t)(t + run) * c.nkv + kvh;
         #pragma unroll
-        for (int w = 0; w < 4; w++) mm = fmaxf(mm, sm_ml[(w * ROWS + r) * 2]);
-        const float m_use = mm == -INFINITY ? 0.f : mm;
-        float acc = 0.f, ll = 0.f;
-        #pragma unroll
-        for (int w = 0; w < 4; w++) {
-            const float a = exp2f(sm_ml[(w * ROWS + r) * 2] - m_use);
-            acc += sm_o[(w * ROWS + r) * HD + x] * a;
-            ll += sm_ml[(w * ROWS + r) * 2 + 1] * a;
+        for (int r = 0; r < 2; r++) {
+            l_i[r] += __shfl_xor_sync(0xffffffffu, l_i[r], 1);
+            l_i[r] += __shfl_xor_sync(0xffffffffu, l_i[r], 2);
         }
-        const size_t slot = ((size_t)(first_seq + rho / G) * nh + kvh * G + rho % G) * n_splits + split;
-        part_o[slot * HD + x] = acc;
-        if (x == 0) { part_ml[slot * 2] = mm; part_ml[slot * 2 + 1] = ll; }
+        if (KQ == 1) {
+            #pragma unroll
+            for (int r = 0; r < 2; r++) {
+                const int rho = rt * 16 + g + 8 * r;
+                if (rho < n_rows) {
+                    float* const to = part_o + (slot * ROWS + rho) * HD + 2 * q2;
+                    #pragma unroll
+                    for (int d = 0; d < HD / 8; d++) *reinterpret_cast<float2*>(to + d * 8) = make_float2(acc[d][2 * r], acc[d][2 * r + 1]);
+                    if (q2 == 0) part_ml[slot * ROWS + rho] = make_float2(m_i[r], l_i[r]);
+                }
+            }
+        } else {
+            // the warps' parts of the keys meet in the space of the tile's last page, which the loader does not have back yet
+            constexpr int LO = HD + 4;
+            static_assert(4 * 16 * (LO + 2) * sizeof(float) <= STAGE * sizeof(bf16), "a page's space holds four warps' results");
+            float* const sm_o = (float*)(ring + (step - 1) % NS * STAGE);        // [4][16][LO]
+            float2* const sm_ml = (float2*)(sm_o + 4 * 16 * LO);                 // [4][16]
+            compute_sync();
+            #pragma unroll
+            for (int r = 0; r < 2; r++) {
+                float* const to = sm_o + (warp * 16 + g + 8 * r) * LO + 2 * q2;
+                #pragma unroll
+                for (int d = 0; d < HD / 8; d++) *reinterpret_cast<float2*>(to + d * 8) = make_float2(acc[d][2 * r], acc[d][2 * r + 1]);
+                if (q2 == 0) sm_ml[warp * 16 + g + 8 * r] = make_float2(m_i[r], l_i[r]);
+            }
+            compute_sync();
+            for (int idx = tid; idx < n_rows * (HD / 4); idx += 128) {
+                const int rho = idx / (HD / 4), x = idx % (HD / 4) * 4;
+                float mm = -INFINITY;
+                #pragma unroll
+                for (int w = 0; w < KQ; w++) mm = fmaxf(mm, sm_ml[w * ROWS + rho].x);
+                const float m_use = mm == -INFINITY ? 0.f : mm;
+                float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+                float ll = 0.f;
+                #pragma unroll
+                for (int w = 0; w < KQ; w++) {
+                    const float2 ml = sm_ml[w * ROWS + rho];
+                    const float a = ik_ex2(ml.x - m_use);
+                    const float4 v = *reinterpret_cast<const float4*>(sm_o + (w * ROWS + rho) * LO + x);
+                    sum.x += v.x * a; sum.y += v.y * a; sum.z += v.z * a; sum.w += v.w * a;
+                    ll += ml.y * a;
+                }
+                *reinterpret_cast<float4*>(part_o + (slot * ROWS + rho) * HD + x) = sum;
+                if (x == 0) part_ml[slot * ROWS + rho] = make_float2(mm, ll);
+            }
+            compute_sync();
+            if (lane == 0) mbar_arrive(&empty[(step - 1) % NS]);
+        }
+    }
+    ik_pdl_launch_dependents();
+}
+
+// Joins a (sequence, head)'s partials in the order of their runs, then the sink.  A warp handles 128 columns of a head at most.
+__global__ void __launch_bounds__(128)
+attn_shared_join_kernel(const float* __restrict__ part_o, const float2* __restrict__ part_ml, bf16* __restrict__ out, const Plan plan, int rows, int heads, int B, int nh,
+                        int nkv, int sink, const float* __restrict__ sink_v) {
+    ik_pdl_wait();
+    ik_pdl_launch_dependents();
+    IK_AFTER_WAIT(part_o);
+    IK_AFTER_WAIT(part_ml);
+    const int b = blockIdx.x, h = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31, G = nh / nkv;
+    if (h >= nh) return;
+    const int2 where = plan.seqs[b];
+    const int in = h % G, t = where.x + in / heads, row = where.y + in % heads, kvh = h / G;
+    const int2 over = where.x >= 0 ? plan.tiles[t] : make_int2(1, 0);
+    const float m_sink = sink ? (sink_v ? sink_v[h] * 1.4426950408889634f : 0.f) : -INFINITY;
+    auto at = [&](int j) { return ((size_t)(t + j) * nkv + kvh) * rows + row; };
+    float mm = m_sink;
+    for (int j = over.x + lane; j <= over.y; j += 32) mm = fmaxf(mm, part_ml[at(j)].x);
+    #pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
+    const float m_use = mm == -INFINITY ? 0.f : mm;
+    for (int x = lane * 4; x < HD; x += 128) {
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        float ll = sink ? ik_ex2(m_sink - m_use) : 0.f;
+        #pragma unroll 4
+        for (int j = over.x; j <= over.y; j++) {
+            const float2 ml = part_ml[at(j)];
+            const float a = ik_ex2(ml.x - m_use);
+            const float4 v = *reinterpret_cast<const float4*>(part_o + at(j) * HD + x);
+            sum.x += v.x * a; sum.y += v.y * a; sum.z += v.z * a; sum.w += v.w * a;
+            ll += ml.y * a;
+        }
+        const float inv = ll > 0.f ? 1.0f / ll : 0.f;
+        ik_st4(out, ((size_t)b * nh + h) * HD + x, make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
     }
 }
 
-// Joins a (sequence, head)'s partials: the shared chunks, then its own, then the sink.
-__global__ void attn_shared_join_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml, bf16* __restrict__ out,
-                                        const int* __restrict__ kv_lens, const int* __restrict__ shared, int table_cols, int nh, int sink,
-                                        const float* __restrict__ sink_v, Cut cut) {
-    ik_pdl_wait();
-    ik_pdl_launch_dependents();
-    const int b = blockIdx.x, h = blockIdx.y;
-    const int pages = min((max(kv_lens[b], 0) + PAGE - 1) / PAGE, table_cols), together = min(max(shared[b], 0), table_cols);
-    const int n_s = chunks_of(together, cut.shared_chunk, cut.n_shared), n_o = chunks_of(pages - min(together, pages), cut.own_chunk, cut.n_own);
-    const size_t base = ((size_t)b * nh + h) * (cut.n_shared + cut.n_own);
-    const float m_sink = sink ? (sink_v ? sink_v[h] * 1.4426950408889634f : 0.f) : -INFINITY;
-    auto at = [&](int i) { return base + (i < n_s ? i : cut.n_shared + i - n_s); };
-    float mm = m_sink;
-    for (int i = 0; i < n_s + n_o; i++) mm = fmaxf(mm, part_ml[at(i) * 2]);
-    const float m_use = mm == -INFINITY ? 0.f : mm;
-    for (int x = threadIdx.x; x < HD; x += blockDim.x) {
-        float acc = 0.f, ll = sink ? exp2f(m_sink - m_use) : 0.f;
-        for (int i = 0; i < n_s + n_o; i++) {
-            const float a = exp2f(part_ml[at(i) * 2] - m_use);
-            acc += part_o[at(i) * HD + x] * a;
-            ll += part_ml[at(i) * 2 + 1] * a;
-        }
-        out[((size_t)b * nh + h) * HD + x] = __float2bfloat16_rn(mm == -INFINITY ? 0.f : acc / ll);
-    }
+template <int RT>
+int launch(const void* q, const void* k_pages, const void* v_pages, void* out, float* scratch, const Call& c, const Plan& plan, float sc_a, float sc_b, int sink,
+           const float* sink_v, int n_pages, int* status, cudaStream_t stream) {
+    const size_t slots = (size_t)(c.n_tiles + c.runs) * c.nkv * 16 * RT;
+    float2* const part_ml = (float2*)(scratch + slots * HD);
+    const size_t smem = (size_t)NS * STAGE * sizeof(bf16) + (size_t)(c.n_tiles + c.B) * sizeof(int);
+    auto kern = attn_shared_kernel<RT>;
+    // one amount whatever the call needs: the attribute belongs to the kernel, and several host threads may launch it
+    const int most = NS * STAGE * (int)sizeof(bf16) + (TILES + SEQS) * (int)sizeof(int);
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+    if (e != cudaSuccess) return (int)e;
+    IK_RETURN_IF_ERROR(ik_launch(kern, dim3(c.runs, c.nkv), THREADS, smem, stream, (const bf16*)q, (const bf16*)k_pages, (const bf16*)v_pages, scratch, part_ml, c, plan,
+                                 sc_a, sc_b, n_pages, status));
+    IK_RETURN_IF_ERROR(ik_launch_family(IK_FAMILY_ATTENTION_MERGE, attn_shared_join_kernel, dim3(c.B, (c.nh + 3) / 4), 128, 0, stream, (const float*)scratch,
+                                        (const float2*)part_ml, (bf16*)out, plan, 16 * RT, c.heads, c.B, c.nh, c.nkv, sink, sink_v));
+    IK_LAUNCH_STATUS();
+}
+
+// How a call is cut into tiles and runs; RT, or a negative status.
+int cut(Call& c, int n_groups, int max_members, int B, int nh, int nkv) {
+    c.n_groups = n_groups; c.B = B; c.nh = nh; c.nkv = nkv; c.G = nh / nkv;
+    const long long rows = (long long)max_members * c.G;
+    const int rt = rows <= 16 ? 1 : rows <= 32 ? 2 : 4, most = 16 * rt;
+    c.heads = c.G < most ? c.G : most;
+    c.head_parts = (c.G + c.heads - 1) / c.heads;
+    c.members = most / c.heads < max_members ? most / c.heads : max_members;
+    const long long per = (long long)((max_members + c.members - 1) / c.members) * c.head_parts;
+    if (per * n_groups > TILES || B > SEQS || nkv > 65535) return IK_UNSUPPORTED;
+    c.tiles_per_group = (int)per;
+    c.n_tiles = (int)per * n_groups;
+    const int runs = BLOCKS * ik_sm_count() / nkv;
+    c.runs = runs > 1 ? runs : 1;
+    return rt;
 }
 
 }  // namespace
 
 IK_EXPORT int ik_attn_shared_head_dim() { return HD; }
+// Sites of the kernel's waits: 41 = loader for a page's space, 42 = computing warps for a page.
+IK_EXPORT int ik_attn_shared_take_wait_record(int* out4) { return ik_take_wait_record(out4); }
 
-// part_o: [B, nh, n_shared + n_own, HD] floats, part_ml: [B, nh, n_shared + n_own, 2] floats, both owned by the caller.  starts: [n_groups + 1], shared: [B], on the
-// device; max_members: no group is larger (rows beyond it would be left out).
-IK_EXPORT int ik_attn_shared(const void* q, const void* k_pages, const void* v_pages, void* out, float* part_o, float* part_ml, const int* kv_lens,
-                             const int* table, int table_stride, int table_cols, const int* starts, const int* shared, int n_groups, int max_members, int B,
-                             int nh, int nkv, float scale, float softcap, int sink, const float* sink_v, int page_size, int n_pages, int shared_chunk,
-                             int n_shared, int own_chunk, int n_own, int* status, cudaStream_t stream) {
+// Bytes of scratch of a call, or a negative status where there are more tiles or sequences than a launch takes.
+IK_EXPORT long long ik_attn_shared_scratch(int n_groups, int max_members, int B, int nh, int nkv) {
+    if (n_groups <= 0 || max_members <= 0 || max_members > B || B <= 0 || nh <= 0 || nkv <= 0 || nh % nkv) return IK_BAD_ARGUMENT;
+    Call c;
+    const int rt = cut(c, n_groups, max_members, B, nh, nkv);
+    if (rt < 0) return rt;
+    return (long long)(c.n_tiles + c.runs) * nkv * 16 * rt * (HD + 2) * 4 + ((long long)B + c.n_tiles) * 8;
+}
+
+// scratch: ik_attn_shared_scratch bytes on 16 bytes.  starts: [n_groups + 1], shared: [B], on the device; max_members: no group is larger (what is beyond is left out).
+IK_EXPORT int ik_attn_shared(const void* q, const void* k_pages, const void* v_pages, void* out, void* scratch, const int* kv_lens, const int* table, int table_stride,
+                             int table_cols, const int* starts, const int* shared, int n_groups, int max_members, int B, int nh, int nkv, float scale, float softcap,
+                             int sink, const float* sink_v, int page_size, int n_pages, int* status, cudaStream_t stream) {
     const float sc_a = softcap > 0.f ? scale / softcap : scale * 1.4426950408889634f, sc_b = softcap > 0.f ? softcap * 1.4426950408889634f : 0.f;
-    if (B <= 0 || nh <= 0 || nkv <= 0 || nh % nkv || page_size != PAGE || n_groups < 0 || max_members <= 0 || max_members > B || shared_chunk <= 0 || own_chunk <= 0 ||
-        n_shared <= 0 || n_own <= 0 || nkv > 65535 || nh > 65535 || table_cols <= 0 || table_stride < table_cols || n_pages <= 0)
+    if (B <= 0 || nh <= 0 || nkv <= 0 || nh % nkv || page_size != PAGE || n_groups <= 0 || max_members <= 0 || max_members > B || nh > 4 * 65535 || table_cols <= 0 ||
+        table_stride < table_cols || n_pages <= 0 || ((uintptr_t)scratch & 15))
         return IK_BAD_ARGUMENT;
-    if (((uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages) & 15) return IK_UNSUPPORTED;
-    const int G = nh / nkv, row_tiles = (max_members * G + ROWS - 1) / ROWS;
-    const Cut cut{shared_chunk, n_shared, own_chunk, n_own};
-    const long long blocks = (long long)n_groups * row_tiles * n_shared + (long long)B * ((G + ROWS - 1) / ROWS) * n_own;
-    if (blocks > 0x7fffffff) return IK_UNSUPPORTED;
-    const size_t q_bytes = (size_t)ROWS * LD * sizeof(bf16), stage_bytes = (size_t)2 * PAGE * LD * sizeof(bf16);
-    const size_t merge_bytes = (size_t)4 * ROWS * (HD + 2) * sizeof(float);
-    constexpr int NS = HD <= 64 ? 4 : HD <= 128 ? 2 : 2;
-    const size_t smem = q_bytes + (NS * stage_bytes > merge_bytes ? NS * stage_bytes : merge_bytes);
-    auto kern = attn_shared_kernel<NS>;
-    if (smem > 48 * 1024) {
-        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e != cudaSuccess) return (int)e;
-    }
-    IK_RETURN_IF_ERROR(ik_launch(kern, dim3((unsigned)blocks, nkv), 128, smem, stream, (const bf16*)q, (const bf16*)k_pages, (const bf16*)v_pages, part_o, part_ml,
-                                 kv_lens, table, table_stride, table_cols, starts, shared, n_groups, row_tiles, B, nh, nkv, sc_a, sc_b, n_pages, cut, status));
-    IK_RETURN_IF_ERROR(ik_launch_family(IK_FAMILY_ATTENTION_MERGE, attn_shared_join_kernel, dim3(B, nh), HD < 128 ? HD : 128, 0, stream, (const float*)part_o,
-                                        (const float*)part_ml, (bf16*)out, kv_lens, shared, table_cols, nh, sink, sink_v, cut));
-    IK_LAUNCH_STATUS();
+    if (((uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)out) & 15) return IK_UNSUPPORTED;
+    Call c;
+    c.kv_lens = kv_lens; c.table = table; c.starts = starts; c.shared = shared; c.table_stride = table_stride; c.table_cols = table_cols;
+    const int rt = cut(c, n_groups, max_members, B, nh, nkv);
+    if (rt < 0) return rt;
+    const size_t parts = (size_t)(c.n_tiles + c.runs) * nkv * 16 * rt * (HD + 2);
+    int2* const seqs = (int2*)((float*)scratch + parts);
+    const Plan plan{seqs, seqs + B};
+    if (rt == 1) return launch<1>(q, k_pages, v_pages, out, (float*)scratch, c, plan, sc_a, sc_b, sink, sink_v, n_pages, status, stream);
+    if (rt == 2) return launch<2>(q, k_pages, v_pages, out, (float*)scratch, c, plan, sc_a, sc_b, sink, sink_v, n_pages, status, stream);
+    return launch<4>(q, k_pages, v_pages, out, (float*)scratch, c, plan, sc_a, sc_b, sink, sink_v, n_pages, status, stream);
 }

@@ -5,11 +5,11 @@ declared outputs.  A non-zero status from the library raises ``KernelError``.
 """
 from __future__ import annotations
 
+import array
 import ctypes
 import os
 from typing import Optional
 
-import numpy as np
 import torch
 
 from . import build
@@ -35,8 +35,12 @@ def _ptr(t: Optional[torch.Tensor]) -> int:
     return 0 if t is None else t.data_ptr()
 
 
+_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+
+
 def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    """The current stream of the current device.  (Asked for without a ``torch.cuda.Stream`` object around it, which costs 3 us a call.)"""
+    return _raw_stream(_current_device())
 
 
 def _need(t: torch.Tensor, name: str, dtype=None, contiguous: bool = True) -> None:
@@ -1144,6 +1148,8 @@ def wait_records() -> str:
     from . import attention_bf16
     for hd, m in attention_bf16._modules.items():
         takers.append((f"attention (head size {hd})", m.ik_attn_take_wait_record))
+    for hd, m in attention_bf16._shared_modules.items():
+        takers.append((f"attention behind shared pages (head size {hd})", m.ik_attn_shared_take_wait_record))
     for name, take in takers:
         if take(rec) == 0 and rec[0] != 0:
             found.append(f"{name}: wait site {rec[0]}, block {rec[1]}, count {rec[2]}, parity {rec[3]}")
@@ -1243,8 +1249,8 @@ def _search_lib():
 
 
 def _here(t: torch.Tensor, name: str) -> None:
-    if t.get_device() != torch.cuda.current_device():
-        raise KernelError(f"{name} is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+    if t.get_device() != _current_device():
+        raise KernelError(f"{name} is on {t.device}, the current device is cuda:{_current_device()}")
 
 
 BEAMS_MOST, BEAM_OUT_MOST, BEAM_VOCAB_MOST = 16, 32, 1 << 20
@@ -1278,28 +1284,29 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n_out: int, out: Opt
             raise KernelError(f"beam_select: out must be [3, {R}, {n_out}], found {tuple(out.shape)}")
     need = R * K * -(-V // 1024) * 16
     scratch = torch.empty(need, dtype=torch.uint8, device=logits.device)
-    s, b, v = out.unbind(0)
+    at, part = out.data_ptr(), 4 * R * n_out
     _work(f"beam select {R}x{K}x{V}", R * K * V * 4 + need)
-    _check(_search_lib().ik_beam_select(_ptr(logits), logits.stride(0), _ptr(scores), R, K, V, n_out, _ptr(scratch), need, _ptr(s), _ptr(b), _ptr(v), _stream()),
+    _check(_search_lib().ik_beam_select(logits.data_ptr(), logits.stride(0), scores.data_ptr(), R, K, V, n_out, scratch.data_ptr(), need, at, at + part, at + 2 * part, _stream()),
            "beam_select", kernels=2)
+    s, b, v = out.unbind(0)
     return s.view(torch.float32), b, v
 
 
-def copy_moves(src, dst, positions, rows: int, page: int) -> np.ndarray:
-    """The moves of one job of ``copy_rows`` as [n, 3] (source, destination, positions), checked."""
+def copy_moves(src, dst, positions, rows: int, page: int) -> list:
+    """The moves of one job of ``copy_rows`` as a flat list (source, destination, positions, source, ...), checked."""
     n = len(src)
     if len(dst) != n or (positions is not None and len(positions) != n):
         raise KernelError(f"copy_rows: {n} sources, {len(dst)} destinations" + ("" if positions is None else f", {len(positions)} numbers of positions"))
-    m = np.empty((n, 3), dtype=np.int64)
-    m[:, 0], m[:, 1], m[:, 2] = src, dst, 1 if positions is None else positions
-    if n and (m[:, :2].min() < 0 or m[:, :2].max() >= rows):
+    if n == 0:
+        return []
+    if min(src) < 0 or min(dst) < 0 or max(src) >= rows or max(dst) >= rows:
         raise KernelError(f"copy_rows: a row is outside the tensor's {rows}")
-    if n and (m[:, 2].min() < 0 or m[:, 2].max() > page):
+    if positions is not None and (min(positions) < 0 or max(positions) > page):
         raise KernelError(f"copy_rows: a number of positions is outside [0, {page}]")
-    to = set(m[:, 1].tolist())
-    if len(to) != n or not to.isdisjoint(m[:, 0].tolist()):
+    to = set(dst)
+    if len(to) != n or not to.isdisjoint(src):
         raise KernelError("copy_rows: a row is written twice, or both read and written")
-    return m
+    return [x for move in zip(src, dst, positions if positions is not None else (1,) * n) for x in move]
 
 
 def copy_rows(jobs) -> None:
@@ -1309,53 +1316,50 @@ def copy_rows(jobs) -> None:
     src, dst and positions are host integers.  A row is not written twice, and none is both read and written: such a job is refused, and so are rows out of range
     and jobs whose tensors overlap.  On refusal nothing has been copied."""
     jobs = list(jobs)                              # the lists below are told apart by identity: they have to live until the end
-    table, moves, spans, nbytes = [], [], [], 0
-    n_moves = 0
-    seen = {}
+    table, moves, spans, seen, n_jobs, nbytes = [], [], [], {}, 0, 0
     for t, src, dst, positions in jobs:
         if not t.is_cuda:
             raise KernelError("copy_rows: a tensor must be a CUDA tensor (there is no CPU path)")
-        if t.dim() < 2 or (positions is not None and t.dim() < 4):
+        shape, strides, size = t.shape, t.stride(), t.element_size()
+        if len(shape) < 2 or (positions is not None and len(shape) < 4):
             raise KernelError("copy_rows: a tensor is [entries, rows, ...], with positions [entries, rows, heads, page, ...]")
         _here(t, "copy_rows: a tensor")
-        n = len(src)
-        if n == len(dst) == 0 or t.numel() == 0:
+        if len(src) == len(dst) == 0 or t.numel() == 0:
             continue
-        shape, strides, size = t.shape, t.stride(), t.element_size()
-        inner = 1
-        for d in range(t.dim() - 1, 1, -1):
-            if shape[d] != 1 and strides[d] != inner:
-                raise KernelError("copy_rows: behind its first two dimensions a tensor must be contiguous")
-            inner *= shape[d]
-        fine = (shape[1] == 1 or strides[1] >= inner) and (shape[0] == 1 or strides[0] >= (shape[1] - 1) * strides[1] + inner
-                                                           or (strides[0] >= inner and strides[1] >= (shape[0] - 1) * strides[0] + inner))
-        if not fine or size % 2:
-            raise KernelError("copy_rows: a tensor's rows may not overlap, and an element has 2, 4, 8 or 16 bytes")
-        page = 1 if positions is None else shape[3]
+        inner = t.numel() // (shape[0] * shape[1])
+        if not t.is_contiguous():
+            step = 1
+            for n, stride in zip(shape[:1:-1], strides[:1:-1]):
+                if n != 1 and stride != step:
+                    raise KernelError("copy_rows: behind its first two dimensions a tensor must be contiguous")
+                step *= n
+            if not ((shape[1] == 1 or strides[1] >= inner) and (shape[0] == 1 or strides[0] >= (shape[1] - 1) * strides[1] + inner
+                                                                or (strides[0] >= inner and strides[1] >= (shape[0] - 1) * strides[0] + inner))):
+                raise KernelError("copy_rows: a tensor's rows may not overlap")
+        if size % 2:
+            raise KernelError("copy_rows: an element must have 2, 4, 8 or 16 bytes")
+        heads, page = (1, 1) if positions is None else (shape[2], shape[3])
         key = (id(src), id(dst), id(positions), shape[1], page)
         at = seen.get(key)
         if at is None:
-            m = copy_moves(src, dst, positions, shape[1], page)
-            at = seen[key] = n_moves
-            moves.append(m)
-            n_moves += n
-        heads = 1 if positions is None else shape[2]
-        per_head = inner // heads * size
-        lo = t.data_ptr()
+            at = seen[key] = len(moves) // 3
+            moves += copy_moves(src, dst, positions, shape[1], page)
+        lo, per_head = t.data_ptr(), inner // heads * size
         spans.append((lo, lo + ((shape[0] - 1) * strides[0] + (shape[1] - 1) * strides[1] + inner) * size))
-        table.append((lo, shape[0], strides[0] * size, shape[1], strides[1] * size, heads, per_head, per_head // page, at, n))
+        table += (lo, shape[0], strides[0] * size, shape[1], strides[1] * size, heads, per_head, per_head // page, at, len(src))
+        n_jobs += 1
         if _profile is not None:
-            nbytes += 2 * shape[0] * heads * (per_head // page) * int(moves[-1][:, 2].sum())
-    if not table:
+            nbytes += 2 * shape[0] * heads * (per_head // page) * sum(moves[3 * at + 2:3 * (at + len(src)):3])
+    if not n_jobs:
         return
-    spans.sort()
-    for a, b in zip(spans, spans[1:]):
-        if b[0] < a[1]:
-            raise KernelError("copy_rows: two jobs' tensors overlap")
-    j = np.array(table, dtype=np.int64)
-    m = (moves[0] if len(moves) == 1 else np.concatenate(moves)).astype(np.int32)
-    _work(f"copy rows {n_moves} moves in {len(table)} tensors", nbytes)
-    _check(_search_lib().ik_copy_rows(j.ctypes.data, len(table), m.ctypes.data, len(m), _stream()), "copy_rows")
+    if n_jobs > 1:
+        spans.sort()
+        for a, b in zip(spans, spans[1:]):
+            if b[0] < a[1]:
+                raise KernelError("copy_rows: two jobs' tensors overlap")
+    j, m = array.array("q", table), array.array("i", moves)
+    _work(f"copy rows {len(moves) // 3} moves in {n_jobs} tensors", nbytes)
+    _check(_search_lib().ik_copy_rows(j.buffer_info()[0], n_jobs, m.buffer_info()[0], len(moves) // 3, _stream()), "copy_rows")
 
 
 # ---------------------------------------------------------------------------------------------

@@ -196,8 +196,8 @@ def test_the_cache_forks_without_a_device():
 
 
 def test_lists_of_moves_are_checked():
-    assert copy_moves([1, 1], (2, 3), [4, 0], 4, 64).tolist() == [[1, 2, 4], [1, 3, 0]]
-    assert copy_moves([], [], None, 4, 1).shape == (0, 3)
+    assert copy_moves([1, 1], (2, 3), [4, 0], 4, 64) == [1, 2, 4, 1, 3, 0] and copy_moves([1, 0], [2, 3], None, 4, 1) == [1, 2, 1, 0, 3, 1]
+    assert copy_moves([], [], None, 4, 1) == []
     for bad in (([0], [1, 2], None), ([0], [4], None), ([-1], [1], None), ([0, 1], [2, 2], None), ([0, 1], [1, 2], None), ([3], [3], None), ([0], [1], [65]), ([0], [1], [-1]),
                 ([0], [1], [1, 2])):
         with pytest.raises(KernelError):

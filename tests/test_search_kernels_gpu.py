@@ -1,6 +1,7 @@
 """The kernels of a search over beams and of forked sequences against plain 64-bit forms: the choice of continuations, the copies of pages and
 states, attention behind shared pages."""
 import math
+import random
 
 import pytest
 import torch
@@ -279,7 +280,7 @@ def layout(members, shared, lens, seed, extra=3):
     return table, total
 
 
-def run_shared(nh, nkv, hd, members, shared, lens, seed=0, softcap=0.0, sink=False, chunks=None, scale=None, garbage=True, bounds=None):
+def run_shared(nh, nkv, hd, members, shared, lens, seed=0, softcap=0.0, sink=False, scale=None, garbage=True, bounds=None):
     from ithaca_b200.csrc import attention_bf16
     g = gen(seed + hd)
     table, total = layout(members, shared, lens, seed)
@@ -297,7 +298,7 @@ def run_shared(nh, nkv, hd, members, shared, lens, seed=0, softcap=0.0, sink=Fal
     owns = [-(-n // 64) - s for n, s in zip(lens, per)]
     got = attention_bf16.decode_shared(q.to(DEV), k.to(DEV), v.to(DEV), torch.tensor(lens, dtype=torch.int32, device=DEV), table.to(DEV), starts.to(DEV),
                                        torch.tensor(per, dtype=torch.int32, device=DEV), len(members), max(members), *(bounds or (max(shared), max(owns))), nh, scale, status,
-                                       softcap=softcap, sink=sink.to(DEV) if torch.is_tensor(sink) else sink, chunks=chunks).cpu().double().view(B, nh, hd)
+                                       softcap=softcap, sink=sink.to(DEV) if torch.is_tensor(sink) else sink).cpu().double().view(B, nh, hd)
     assert status.item() == 0
     for b, n in enumerate(lens):
         if n == 0:
@@ -336,10 +337,16 @@ def test_attention_behind_shared_pages(nh, nkv, hd, members, shared, lens):
     run_shared(nh, nkv, hd, members, shared, lens, seed=len(lens))
 
 
-@pytest.mark.parametrize("chunks", [(1, 1), (2, 1), (3, 5), (64, 64)])
-def test_every_cut_of_the_pages(chunks):
-    run_shared(8, 2, 64, [3, 2], [7, 4], [449, 500, 700, 257, 300], seed=4, chunks=chunks)
-    run_shared(8, 2, 128, [3, 2], [7, 4], [449, 500, 700, 257, 300], seed=5, chunks=chunks)
+@pytest.mark.parametrize("nh,nkv,hd", [(40, 40, 128), (64, 64, 64), (80, 1, 64), (40, 1, 128), (20, 1, 64), (4, 4, 16), (24, 2, 96), (148, 148, 32)])
+@pytest.mark.parametrize("seed", range(4))
+def test_many_groups_of_all_sizes(nh, nkv, hd, seed):
+    """Runs of pages that end inside tiles, cover several, begin among shared pages or among a member's own; more heads per kv head than a tile has rows; groups
+    of more members than fit one."""
+    r = random.Random(seed)
+    members = [r.choice([1, 1, 2, 3, 7, 20]) for _ in range(r.choice([1, 5, 14]))]
+    shared = [r.choice([0, 1, 2, 9]) if m > 1 else r.choice([0, 0, 3]) for m in members]
+    lens = [s * 64 + r.choice([0, 1, 3, 64, 65, 200, r.randint(0, 700)]) for m, s in zip(members, shared) for _ in range(m)]
+    run_shared(nh, nkv, hd, members, shared, lens, seed=seed)
 
 
 def test_bounds_that_are_too_small_cost_time_only():
@@ -400,7 +407,7 @@ def test_shared_attention_refuses():
                 n_groups=1, max_members=4, shared_bound=1, own_bound=1, n_heads=4, scale=0.125, status=None)
     attention_bf16.decode_shared(**good)
     for bad in (dict(q=q.float()), dict(k_pages=k.float()), dict(v_pages=k[:5]), dict(n_heads=3), dict(q=q[:3]), dict(starts=ints(0, 2, 4)), dict(shared=ints(1, 1)), dict(max_members=0),
-                dict(max_members=5), dict(table=good["table"][:3]), dict(table=good["table"].long()), dict(kv_lens=good["kv_lens"].cpu()), dict(k_pages=k[:, :, :32], v_pages=k[:, :, :32]),
+                dict(max_members=5), dict(n_groups=0, starts=ints(0)), dict(table=good["table"][:3]), dict(table=good["table"].long()), dict(kv_lens=good["kv_lens"].cpu()), dict(k_pages=k[:, :, :32], v_pages=k[:, :, :32]),
                 dict(sink=torch.zeros(3, device=DEV)), dict(k_pages=k[..., :24], v_pages=k[..., :24])):
         with pytest.raises(o.KernelError):
             attention_bf16.decode_shared(**{**good, **bad})
