@@ -35,6 +35,7 @@ constexpr int STAGE = 2 * PAGE * LD;       // keys and values of a page, in elem
 constexpr int NS = HD <= 64 ? 4 : 3;       // pages of the ring: 104 KB at head size 128, two blocks to an SM
 constexpr int BLOCKS = HD <= 128 ? 2 : 1;  // blocks of an SM
 constexpr int THREADS = 160;               // four computing warps, one that loads
+constexpr int JOIN_FAMILY = IK_FAMILY_ELEMENTWISE;
 constexpr int TILES = 1024, SEQS = 1024;   // most tiles and sequences of a launch
 constexpr int LEAST = 2;                   // least pages of a run: a block's set-up and its partial cost about as much as two
 static_assert(HD % 16 == 0 && HD >= 16 && HD <= 256, "head size must be a multiple of 16 up to 256");
@@ -381,40 +382,53 @@ attn_shared_kernel(const bf16* __restrict__ q, const bf16* __restrict__ k_pages,
     ik_pdl_launch_dependents();
 }
 
-// Joins a (sequence, head)'s partials in the order of their runs, then the sink.  A warp handles 128 columns of a head at most.
-__global__ void __launch_bounds__(128)
-attn_shared_join_kernel(const float* __restrict__ part_o, const float2* __restrict__ part_ml, bf16* __restrict__ out, const Plan plan, int rows, int heads, int B, int nh,
+// Joins a (sequence, head)'s partials, then the sink: a block each, whose groups of HD / 4 threads take every JG-th run and are summed in their order.
+constexpr int JV = HD / 4, JG = HD <= 128 ? 128 / JV : 2, JT = JV * JG;
+__global__ void __launch_bounds__(JT)
+attn_shared_join_kernel(const float* __restrict__ part_o, const float2* __restrict__ part_ml, bf16* __restrict__ out, const Plan plan, int rows, int heads, int nh,
                         int nkv, int sink, const float* __restrict__ sink_v) {
+    __shared__ float4 sums[JG][JV];
+    __shared__ float2 ml_of[JG];
     ik_pdl_wait();
     ik_pdl_launch_dependents();
     IK_AFTER_WAIT(part_o);
     IK_AFTER_WAIT(part_ml);
-    const int b = blockIdx.x, h = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31, G = nh / nkv;
-    if (h >= nh) return;
+    const int b = blockIdx.x, h = blockIdx.y, G = nh / nkv, grp = threadIdx.x / JV, x = threadIdx.x % JV;
     const int2 where = plan.seqs[b];
     const int in = h % G, t = where.x + in / heads, row = where.y + in % heads, kvh = h / G;
     const int2 over = where.x >= 0 ? plan.tiles[t] : make_int2(1, 0);
-    const float m_sink = sink ? (sink_v ? sink_v[h] * 1.4426950408889634f : 0.f) : -INFINITY;
-    auto at = [&](int j) { return ((size_t)(t + j) * nkv + kvh) * rows + row; };
-    float mm = m_sink;
-    for (int j = over.x + lane; j <= over.y; j += 32) mm = fmaxf(mm, part_ml[at(j)].x);
-    #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
-    const float m_use = mm == -INFINITY ? 0.f : mm;
-    for (int x = lane * 4; x < HD; x += 128) {
-        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-        float ll = sink ? ik_ex2(m_sink - m_use) : 0.f;
-        #pragma unroll 4
-        for (int j = over.x; j <= over.y; j++) {
-            const float2 ml = part_ml[at(j)];
-            const float a = ik_ex2(ml.x - m_use);
-            const float4 v = *reinterpret_cast<const float4*>(part_o + at(j) * HD + x);
-            sum.x += v.x * a; sum.y += v.y * a; sum.z += v.z * a; sum.w += v.w * a;
-            ll += ml.y * a;
-        }
-        const float inv = ll > 0.f ? 1.0f / ll : 0.f;
-        ik_st4(out, ((size_t)b * nh + h) * HD + x, make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    float m = -INFINITY, l = 0.f;
+    #pragma unroll 4
+    for (int j = over.x + grp; j <= over.y; j += JG) {
+        const size_t at = ((size_t)(t + j) * nkv + kvh) * rows + row;
+        const float2 ml = part_ml[at];
+        const float4 v = *reinterpret_cast<const float4*>(part_o + at * HD + x * 4);
+        const float m_new = fmaxf(m, ml.x), m_use = m_new == -INFINITY ? 0.f : m_new, a = ik_ex2(m - m_use), w = ik_ex2(ml.x - m_use);
+        sum = make_float4(sum.x * a + v.x * w, sum.y * a + v.y * w, sum.z * a + v.z * w, sum.w * a + v.w * w);
+        l = l * a + ml.y * w;
+        m = m_new;
     }
+    sums[grp][x] = sum;
+    if (x == 0) ml_of[grp] = make_float2(m, l);
+    __syncthreads();
+    if (grp != 0) return;
+    const float m_sink = sink ? (sink_v ? sink_v[h] * 1.4426950408889634f : 0.f) : -INFINITY;
+    float mm = m_sink;
+    #pragma unroll
+    for (int i = 0; i < JG; i++) mm = fmaxf(mm, ml_of[i].x);
+    const float m_use = mm == -INFINITY ? 0.f : mm;
+    sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    l = sink ? ik_ex2(m_sink - m_use) : 0.f;
+    #pragma unroll
+    for (int i = 0; i < JG; i++) {
+        const float w = ik_ex2(ml_of[i].x - m_use);
+        const float4 v = sums[i][x];
+        sum.x += v.x * w; sum.y += v.y * w; sum.z += v.z * w; sum.w += v.w * w;
+        l += ml_of[i].y * w;
+    }
+    const float inv = l > 0.f ? 1.0f / l : 0.f;                        // (no keys: zeros; a sum that is not a number is passed on below)
+    ik_st4(out, ((size_t)b * nh + h) * HD + x * 4, l == l ? make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv) : make_float4(l, l, l, l));
 }
 
 template <int RT>
@@ -430,8 +444,8 @@ int launch(const void* q, const void* k_pages, const void* v_pages, void* out, f
     if (e != cudaSuccess) return (int)e;
     IK_RETURN_IF_ERROR(ik_launch(kern, dim3(c.runs, c.nkv), THREADS, smem, stream, (const bf16*)q, (const bf16*)k_pages, (const bf16*)v_pages, scratch, part_ml, c, plan,
                                  sc_a, sc_b, n_pages, status));
-    IK_RETURN_IF_ERROR(ik_launch_family(IK_FAMILY_ATTENTION_MERGE, attn_shared_join_kernel, dim3(c.B, (c.nh + 3) / 4), 128, 0, stream, (const float*)scratch,
-                                        (const float2*)part_ml, (bf16*)out, plan, 16 * RT, c.heads, c.B, c.nh, c.nkv, sink, sink_v));
+    IK_RETURN_IF_ERROR(ik_launch_family(JOIN_FAMILY, attn_shared_join_kernel, dim3(c.B, c.nh), JT, 0, stream, (const float*)scratch, (const float2*)part_ml, (bf16*)out,
+                                        plan, 16 * RT, c.heads, c.nh, c.nkv, sink, sink_v));
     IK_LAUNCH_STATUS();
 }
 
@@ -472,7 +486,7 @@ IK_EXPORT int ik_attn_shared(const void* q, const void* k_pages, const void* v_p
                              int table_cols, const int* starts, const int* shared, int n_groups, int max_members, int B, int nh, int nkv, float scale, float softcap,
                              int sink, const float* sink_v, int page_size, int n_pages, int* status, cudaStream_t stream) {
     const float sc_a = softcap > 0.f ? scale / softcap : scale * 1.4426950408889634f, sc_b = softcap > 0.f ? softcap * 1.4426950408889634f : 0.f;
-    if (B <= 0 || nh <= 0 || nkv <= 0 || nh % nkv || page_size != PAGE || n_groups <= 0 || max_members <= 0 || max_members > B || nh > 4 * 65535 || table_cols <= 0 ||
+    if (B <= 0 || nh <= 0 || nkv <= 0 || nh % nkv || page_size != PAGE || n_groups <= 0 || max_members <= 0 || max_members > B || nh > 65535 || table_cols <= 0 ||
         table_stride < table_cols || n_pages <= 0 || ((uintptr_t)scratch & 15))
         return IK_BAD_ARGUMENT;
     if (((uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)out) & 15) return IK_UNSUPPORTED;
