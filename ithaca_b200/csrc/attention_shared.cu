@@ -11,9 +11,12 @@
 // maximum, sum) and goes on; a second kernel joins each row's partials in the order of their runs.  Run j's partial of tile t is kept at t + j: each new
 // partial is one tile or one run further, so the numbers are distinct and dense.
 //
-// A block: one warp brings pages into a ring of shared memory (cp.async), four compute on mma.sync m16n8k16 tiles.  A warp owns 16 rows and 64 / KQ
-// of a page's keys (RT = 1, 2 or 4 tiles of 16 rows, KQ = 4 / RT), with running maximum and sum as floats, base 2; the warps of equal rows are merged at the
-// end of a tile.  Probabilities are rounded to bfloat16 for the second product, as the other attention kernels do.
+// A block: one warp brings pages into a ring of shared memory (by TMA with the 128-byte swizzle for head sizes that are multiples of 64, else by cp.async into
+// padded rows: a warp takes 1,700 cycles to issue a page of head size 128 that way, one thread a hundred by TMA), four compute on mma.sync m16n8k16 tiles.
+// A warp owns 16 rows and all 64 keys of a page, with running maximum and sum as floats, base 2.  RT = 1, 2 or 4 warps share a page, one for each 16
+// of a tile's rows, and PG = 4 / RT such groups take turns with the pages: what a page costs besides its products (waits, the maximum's way across lanes) passes
+// on several pages at once.  (With every page's keys shared out to the four warps a page of head size 64 took 2,000 cycles, more than its bytes.)  The groups'
+// results are merged at the end of a tile.  Probabilities are rounded to bfloat16 for the second product, as the other attention kernels do.
 //
 // Keys behind a sequence's length are masked by position and their values are brought as zeros, so what lies in the unused part of a page never
 // matters.  A page index outside the pool sets *status and is not followed.  A sequence without keys gets zeros.
@@ -28,19 +31,21 @@
 
 namespace {
 
+typedef __nv_bfloat16 bf16;
+
 constexpr int HD = IK_HD;
 constexpr int PAGE = 64;
-constexpr int LD = HD + 8;                 // padded row: consecutive rows fall into different banks
-constexpr int STAGE = 2 * PAGE * LD;       // keys and values of a page, in elements
-constexpr int NS = HD <= 64 ? 4 : 3;       // pages of the ring: 104 KB at head size 128, two blocks to an SM
+constexpr bool TMA = HD % 64 == 0;
+constexpr int LD = TMA ? HD : HD + 8;      // row of a page in shared memory: swizzled blocks of 64 columns, or padded so that consecutive rows fall into different banks
+constexpr int HALF = PAGE * LD, STAGE = 2 * HALF;        // keys (or values) of a page, both, in elements
 constexpr int BLOCKS = HD <= 128 ? 2 : 1;  // blocks of an SM
+constexpr int FIT = 98304 / (STAGE * 2) * (HD <= 128 ? 1 : 2), NS = FIT > 8 ? 8 : FIT < 3 ? 3 : FIT;       // pages of the ring: 96 KB where two blocks share an SM
 constexpr int THREADS = 160;               // four computing warps, one that loads
+constexpr size_t RING = (size_t)NS * STAGE * sizeof(bf16), FIXED = RING + 64 * 8 + 2 * NS * 8 + 8;         // bytes of the ring; with results' maxima and sums, barriers, a flag
 constexpr int JOIN_FAMILY = IK_FAMILY_ELEMENTWISE;
 constexpr int TILES = 1024, SEQS = 1024;   // most tiles and sequences of a launch
 constexpr int LEAST = 2;                   // least pages of a run: a block's set-up and its partial cost about as much as two
 static_assert(HD % 16 == 0 && HD >= 16 && HD <= 256, "head size must be a multiple of 16 up to 256");
-
-typedef __nv_bfloat16 bf16;
 
 __device__ __forceinline__ void cp16(uint32_t smem, const void* gmem, bool valid) {
     const int n = valid ? 16 : 0;
@@ -52,10 +57,10 @@ __device__ __forceinline__ void cp_arrive(uint64_t* bar) {
 }
 __device__ __forceinline__ void compute_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t s) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(s) : "memory");
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(s) : "memory");
 }
 __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t s) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(s) : "memory");
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(s) : "memory");
 }
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
@@ -63,6 +68,11 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// Bytes from a tile's start to the 8 columns number `chunk` of `row`; row7 = row % 8 (rows of 128 bytes, 64 to a block, their 16-byte pieces exchanged by row % 8).
+__device__ __forceinline__ uint32_t piece(int row, int row7, int chunk) {
+    return TMA ? (uint32_t)((chunk >> 3) * PAGE * 128 + row * 128 + (((chunk & 7) ^ row7) << 4)) : (uint32_t)(row * LD + chunk * 8) * 2;
+}
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<uint32_t*>(&v);
@@ -83,14 +93,14 @@ struct Call {
     int runs;
 };
 struct TileOf { int first, last, part, S; };                          // members first <= i < last, part of the heads, pages they share
-__device__ __forceinline__ TileOf tile_of(const Call& c, int t) {
+__device__ __forceinline__ TileOf tile_of(const Call& c, const int* starts, const int* shared, int t) {
     const int g = t / c.tiles_per_group, k = t % c.tiles_per_group;
-    const int a = min(max(c.starts[g], 0), c.B), b = min(max(c.starts[g + 1], a), c.B);
+    const int a = min(max(starts[g], 0), c.B), b = min(max(starts[g + 1], a), c.B);
     TileOf o;
     o.part = k % c.head_parts;
     o.first = min(a + k / c.head_parts * c.members, b);
     o.last = min(o.first + c.members, b);
-    o.S = a < b ? min(max(c.shared[a], 0), c.table_cols) : 0;
+    o.S = a < b ? min(max(shared[a], 0), c.table_cols) : 0;
     return o;
 }
 // pages: how many every sequence has, shared ones included.
@@ -101,10 +111,20 @@ __device__ __forceinline__ int pages_in(const int* pages, const TileOf& o) {
     for (int i = o.first; i < o.last; i++) n += own_pages(pages, o, i);
     return n;
 }
-// Runs in use, the first page of a run, the run of a page.
-__device__ __forceinline__ int runs_of(int pages, int runs) { return min(runs, (pages + LEAST - 1) / LEAST); }
-__device__ __forceinline__ int run_start(int j, int pages, int runs) { return (int)((long long)j * pages / runs); }
-__device__ __forceinline__ int run_of(int page, int pages, int runs) { return (int)((((long long)page + 1) * runs - 1) / pages); }
+// The runs in use: so many of `len` + 1 pages, then of `len`.  The first page of a run, the run of a page.
+struct Cut { int runs, len, longer; };
+__device__ __forceinline__ Cut cut_of(int pages, int most) {
+    Cut c;
+    c.runs = min(most, (pages + LEAST - 1) / LEAST);
+    c.len = pages / max(c.runs, 1);
+    c.longer = pages - c.len * c.runs;
+    return c;
+}
+__device__ __forceinline__ int run_start(const Cut& c, int j) { return j * c.len + min(j, c.longer); }
+__device__ __forceinline__ int run_of(const Cut& c, int page) {
+    const int split = c.longer * (c.len + 1);
+    return page < split ? page / (c.len + 1) : c.longer + (page - split) / c.len;
+}
 
 // The plan that the first block leaves for the join: per sequence its first tile and row, per tile its first and last run (no run: 1, 0).
 struct Plan { int2* seqs; int2* tiles; };
@@ -112,26 +132,39 @@ struct Plan { int2* seqs; int2* tiles; };
 template <int RT>
 __global__ void __launch_bounds__(THREADS, BLOCKS)
 attn_shared_kernel(const bf16* __restrict__ q, const bf16* __restrict__ k_pages, const bf16* __restrict__ v_pages, float* __restrict__ part_o,
-                   float2* __restrict__ part_ml, const Call c, const Plan plan, float scale_log2e, float cap_log2e, int n_pages, int* status) {
-    constexpr int ROWS = 16 * RT, KQ = 4 / RT, KEYS = PAGE / KQ, NB = KEYS / 8, CH = HD / 8;
+                   float2* __restrict__ part_ml, const Call c, const Plan plan, float scale_log2e, float cap_log2e, int n_pages, int* status,
+                   const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
+    constexpr int ROWS = 16 * RT, PG = 4 / RT, NB = PAGE / 8, CH = HD / 8;
     ik_pdl_wait();
-    extern __shared__ __align__(16) unsigned char smem_raw[];
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
     bf16* const ring = (bf16*)smem_raw;                              // [NS][keys, values][PAGE][LD]
-    int* const ends = (int*)(smem_raw + (size_t)NS * STAGE * sizeof(bf16));     // [n_tiles]: pages up to and with a tile
+    float2* const sm_ml = (float2*)(smem_raw + RING);                // [4][16]: maxima and sums
+    uint64_t* const full = (uint64_t*)(sm_ml + 64);                  // [NS]
+    uint64_t* const empty = full + NS;                               // [NS]
+    int& abort_flag = *(int*)(empty + NS);
+    int* const ends = &abort_flag + 2;                               // [n_tiles]: pages up to and with a tile
     int* const pages = ends + c.n_tiles;                             // [B]
-    __shared__ uint64_t full[NS], empty[NS];
-    __shared__ int abort_flag;
+    int* const shared = pages + c.B;                                 // [B]
+    int* const starts = shared + c.B;                                // [n_groups + 1]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, run = blockIdx.x, kvh = blockIdx.y;
 
     if (tid == 0) {
         abort_flag = 0;
         #pragma unroll
-        for (int s = 0; s < NS; s++) { mbar_init(&full[s], 32); mbar_init(&empty[s], 4); }
+        for (int s = 0; s < NS; s++) { mbar_init(&full[s], TMA ? 1 : 32); mbar_init(&empty[s], 4); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    for (int i = tid; i < c.B; i += THREADS) pages[i] = min((max(c.kv_lens[i], 0) + PAGE - 1) / PAGE, c.table_cols);
+    // the block tables, on their way to L2 while the plan is made (all blocks together)
+    for (long long i = (long long)(blockIdx.y * gridDim.x + blockIdx.x) * THREADS + tid; i * 32 < (long long)c.B * c.table_stride; i += (long long)gridDim.x * gridDim.y * THREADS)
+        asm volatile("prefetch.global.L2 [%0];" :: "l"(c.table + min(i * 32, (long long)(c.B - 1) * c.table_stride + c.table_cols - 1)));
+    for (int i = tid; i < c.B; i += THREADS) {
+        shared[i] = c.shared[i];
+        pages[i] = min((max(c.kv_lens[i], 0) + PAGE - 1) / PAGE, c.table_cols);
+    }
+    for (int i = tid; i <= c.n_groups; i += THREADS) starts[i] = c.starts[i];
+    if (TMA && tid == 0 && (smem_u32(smem_raw) & 1023)) { abort_flag = 1; ik_set_status(status, IK_STATUS_SMEM_ALIGN); }
     __syncthreads();
-    for (int t = tid; t < c.n_tiles; t += THREADS) ends[t] = pages_in(pages, tile_of(c, t));
+    for (int t = tid; t < c.n_tiles; t += THREADS) ends[t] = pages_in(pages, tile_of(c, starts, shared, t));
     __syncthreads();
     if (warp == 0) {
         int before = 0;
@@ -144,20 +177,20 @@ attn_shared_kernel(const bf16* __restrict__ q, const bf16* __restrict__ k_pages,
         }
     }
     __syncthreads();
-    const int total = ends[c.n_tiles - 1], runs = total > 0 ? runs_of(total, c.runs) : 0;
+    const Cut cut = cut_of(ends[c.n_tiles - 1], c.runs);
     if (run == 0 && kvh == 0) {
         for (int i = tid; i < c.B; i += THREADS) plan.seqs[i] = make_int2(-1, 0);
         __syncthreads();
         for (int t = tid; t < c.n_tiles; t += THREADS) {
             const int lo = t ? ends[t - 1] : 0, hi = ends[t];
-            plan.tiles[t] = lo < hi ? make_int2(run_of(lo, total, runs), run_of(hi - 1, total, runs)) : make_int2(1, 0);
-            const TileOf o = tile_of(c, t);
+            plan.tiles[t] = lo < hi ? make_int2(run_of(cut, lo), run_of(cut, hi - 1)) : make_int2(1, 0);
+            const TileOf o = tile_of(c, starts, shared, t);
             if (o.part == 0)
                 for (int i = o.first; i < o.last; i++) plan.seqs[i] = make_int2(t, (i - o.first) * c.heads);
         }
     }
-    if (run >= runs) return;
-    const int u_first = run_start(run, total, runs), u_end = run_start(run + 1, total, runs);
+    if (run >= cut.runs || abort_flag) return;
+    const int u_first = run_start(cut, run), u_end = run_start(cut, run + 1);
     int t = 0;
     while (ends[t] <= u_first) t++;
 
@@ -168,7 +201,7 @@ attn_shared_kernel(const bf16* __restrict__ q, const bf16* __restrict__ k_pages,
         for (int u = u_first; u < u_end && alive;) {
             while (ends[t] <= u) t++;
             const int lo = t ? ends[t - 1] : 0, n = min(min(ends[t], u_end) - u, 32);
-            const TileOf o = tile_of(c, t);
+            const TileOf o = tile_of(c, starts, shared, t);
             int page = 0, filled = PAGE;
             if (lane < n) {
                 int i = u + lane - lo, seq = o.first, col = i;
@@ -185,28 +218,46 @@ attn_shared_kernel(const bf16* __restrict__ q, const bf16* __restrict__ k_pages,
                 const int stage = step % NS, pg = __shfl_sync(0xffffffffu, page, l), rows = __shfl_sync(0xffffffffu, filled, l);
                 alive = __all_sync(0xffffffffu, step < NS || mbar_wait(&empty[stage], (step / NS - 1) & 1, &abort_flag, status, IK_WAIT_LIMIT_NS, 41, step));
                 if (!alive) break;
-                const bf16* const kg = k_pages + ((size_t)pg * c.nkv + kvh) * PAGE * HD;
-                const bf16* const vg = v_pages + ((size_t)pg * c.nkv + kvh) * PAGE * HD;
-                const uint32_t to = smem_u32(ring + stage * STAGE);
-                #pragma unroll 8
-                for (int idx = lane; idx < PAGE * CH; idx += 32) cp16(to + (idx / CH * LD + idx % CH * 8) * 2, kg + idx * 8, true);
-                #pragma unroll 8
-                for (int idx = lane; idx < PAGE * CH; idx += 32) cp16(to + (PAGE * LD + idx / CH * LD + idx % CH * 8) * 2, vg + idx * 8, idx / CH < rows);
-                cp_arrive(&full[stage]);
+                bf16* const to = ring + stage * STAGE;
+                if (TMA) {
+                    if (elect_one()) {
+                        mbar_expect_tx(&full[stage], STAGE * sizeof(bf16));
+                        const int y = (pg * c.nkv + kvh) * PAGE;
+                        #pragma unroll
+                        for (int x = 0; x < HD; x += 64) tma_load_2d(to + x * PAGE, &map_k, x, y, &full[stage]);
+                        #pragma unroll
+                        for (int x = 0; x < HD; x += 64) tma_load_2d(to + HALF + x * PAGE, &map_v, x, y, &full[stage]);
+                    }
+                    __syncwarp();
+                } else {
+                    const bf16* const kg = k_pages + ((size_t)pg * c.nkv + kvh) * PAGE * HD;
+                    const bf16* const vg = v_pages + ((size_t)pg * c.nkv + kvh) * PAGE * HD;
+                    const uint32_t at = smem_u32(to);
+                    #pragma unroll 8
+                    for (int idx = lane; idx < PAGE * CH; idx += 32) cp16(at + piece(idx / CH, 0, idx % CH), kg + idx * 8, true);
+                    #pragma unroll 8
+                    for (int idx = lane; idx < PAGE * CH; idx += 32) cp16(at + HALF * 2 + piece(idx / CH, 0, idx % CH), vg + idx * 8, idx / CH < rows);
+                    cp_arrive(&full[stage]);
+                }
             }
             u += n;
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
+        if (TMA && !alive)                                            // what was asked for lands before the block's memory goes (a limit here, too)
+            for (int i = max(0, step - NS); i < step; i++) {
+                const long long c0 = wait_clock();
+                while (!mbar_test(&full[i % NS], (i / NS) & 1) && !wait_ran_out(c0, IK_WAIT_LIMIT_NS)) {}
+            }
         return;
     }
 
     // ---- the computing warps
-    const int g = lane >> 2, q2 = lane & 3, rt = warp % RT, kq = warp / RT;
+    const int g = lane >> 2, q2 = lane & 3, rt = warp % RT, mine = warp / RT;
     int step = 0;
     for (int u = u_first; u < u_end;) {
         while (ends[t] <= u) t++;
         const int lo = t ? ends[t - 1] : 0, stop = min(ends[t], u_end);
-        const TileOf o = tile_of(c, t);
+        const TileOf o = tile_of(c, starts, shared, t);
         const int n_rows = (o.last - o.first) * c.heads;             // rows of this tile (fewer where the last part of the heads is not full)
         int seq_of[2], pos[2];
         const bf16* qrow[2];
@@ -245,9 +296,25 @@ attn_shared_kernel(const bf16* __restrict__ q, const bf16* __restrict__ k_pages,
                 while (own_pages(pages, o, member) == 0) member++;
                 col = o.S;
             }
-            const int stage = step % NS;
+            const int at = own ? col++ : u - lo, stage = step % NS;          // the page's number in the sequence
+            // every warp sees every page arrive and gives it back, its own behind its work: a barrier's phase that a warp had not seen could be
+            // mistaken for the one before it, or be over before the warp looks
             if (!__all_sync(0xffffffffu, mbar_wait(&full[stage], (step / NS) & 1, &abort_flag, status, IK_WAIT_LIMIT_NS, 42, step))) return;
-            const uint32_t ks_ = smem_u32(ring + stage * STAGE + kq * KEYS * LD), vs_ = ks_ + PAGE * LD * 2;
+            if (step % PG != mine) {
+                if (lane == 0 && u + 1 < stop) mbar_arrive(&empty[stage]);
+                continue;
+            }
+            const uint32_t ks_ = smem_u32(ring + stage * STAGE), vs_ = ks_ + HALF * 2;
+            if (TMA && own) {                                         // values behind the last key: zeros (by cp.async they come so)
+                const int from = c.kv_lens[member] - at * PAGE;
+                if (from < PAGE) {
+                    for (int i = lane; i < (PAGE - from) * 8; i += 32)
+                        #pragma unroll
+                        for (int x = 0; x < HD; x += 64) *reinterpret_cast<uint4*>((unsigned char*)(ring + stage * STAGE + HALF + x * PAGE) + from * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+                    __syncwarp();
+                    fence_async();
+                }
+            }
             float s[NB][4];
             #pragma unroll
             for (int n = 0; n < NB; n++)
@@ -258,13 +325,13 @@ attn_shared_kernel(const bf16* __restrict__ q, const bf16* __restrict__ k_pages,
                 #pragma unroll
                 for (int np = 0; np < NB / 2; np++) {
                     uint32_t bfr[4];
-                    ldsm4(bfr, ks_ + (((np * 16 + (lane & 7) + (lane >> 4) * 8) * LD + ks * 16 + ((lane >> 3) & 1) * 8) * 2));
+                    ldsm4(bfr, ks_ + piece(np * 16 + (lane & 7) + (lane >> 4) * 8, lane & 7, ks * 2 + ((lane >> 3) & 1)));
                     mma(s[2 * np], qf[ks], bfr[0], bfr[1]);
                     mma(s[2 * np + 1], qf[ks], bfr[2], bfr[3]);
                 }
             float mx[2] = {-INFINITY, -INFINITY};
             if (own || ends_early) {
-                const int jbase = (own ? col : u - lo) * PAGE + kq * KEYS + 2 * q2;
+                const int jbase = at * PAGE + 2 * q2;
                 #pragma unroll
                 for (int n = 0; n < NB; n++)
                     #pragma unroll
@@ -283,7 +350,6 @@ attn_shared_kernel(const bf16* __restrict__ q, const bf16* __restrict__ k_pages,
                         mx[e >> 1] = fmaxf(mx[e >> 1], s[n][e]);
                     }
             }
-            col += own;
             float alpha[2], rs[2] = {0.f, 0.f};
             #pragma unroll
             for (int r = 0; r < 2; r++) {
@@ -316,13 +382,13 @@ attn_shared_kernel(const bf16* __restrict__ q, const bf16* __restrict__ k_pages,
                 #pragma unroll
                 for (int dp = 0; dp < HD / 16; dp++) {
                     uint32_t bfr[4];
-                    ldsm4t(bfr, vs_ + (((kk * 16 + (lane & 7) + ((lane >> 3) & 1) * 8) * LD + dp * 16 + (lane >> 4) * 8) * 2));
+                    ldsm4t(bfr, vs_ + piece(kk * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, lane & 7, dp * 2 + (lane >> 4)));
                     mma(acc[2 * dp], pa[kk], bfr[0], bfr[1]);
                     mma(acc[2 * dp + 1], pa[kk], bfr[2], bfr[3]);
                 }
             __syncwarp();
             // the last page of a tile is given back behind the merge below, which uses its space
-            if (lane == 0 && (KQ == 1 || u + 1 < stop)) mbar_arrive(&empty[stage]);
+            if (lane == 0 && (PG == 1 || u + 1 < stop)) mbar_arrive(&empty[stage]);
         }
         const size_t slot = (size_t)(t + run) * c.nkv + kvh;
         #pragma unroll
@@ -330,7 +396,7 @@ attn_shared_kernel(const bf16* __restrict__ q, const bf16* __restrict__ k_pages,
             l_i[r] += __shfl_xor_sync(0xffffffffu, l_i[r], 1);
             l_i[r] += __shfl_xor_sync(0xffffffffu, l_i[r], 2);
         }
-        if (KQ == 1) {
+        if (PG == 1) {
             #pragma unroll
             for (int r = 0; r < 2; r++) {
                 const int rho = rt * 16 + g + 8 * r;
@@ -343,16 +409,14 @@ attn_shared_kernel(const bf16* __restrict__ q, const bf16* __restrict__ k_pages,
             }
         } else {
             // the warps' parts of the keys meet in the space of the tile's last page, which the loader does not have back yet
-            constexpr int LO = HD + 4;
-            static_assert(4 * 16 * (LO + 2) * sizeof(float) <= STAGE * sizeof(bf16), "a page's space holds four warps' results");
-            float* const sm_o = (float*)(ring + (step - 1) % NS * STAGE);        // [4][16][LO]
-            float2* const sm_ml = (float2*)(sm_o + 4 * 16 * LO);                 // [4][16]
+            static_assert(4 * 16 * HD * sizeof(float) <= STAGE * sizeof(bf16), "a page's space holds four warps' results");
+            float* const sm_o = (float*)(ring + (step - 1) % NS * STAGE);        // [4][16][HD], fours of columns exchanged by row
             compute_sync();
             #pragma unroll
             for (int r = 0; r < 2; r++) {
-                float* const to = sm_o + (warp * 16 + g + 8 * r) * LO + 2 * q2;
+                float* const to = sm_o + (warp * 16 + g + 8 * r) * HD;
                 #pragma unroll
-                for (int d = 0; d < HD / 8; d++) *reinterpret_cast<float2*>(to + d * 8) = make_float2(acc[d][2 * r], acc[d][2 * r + 1]);
+                for (int d = 0; d < HD / 8; d++) *reinterpret_cast<float2*>(to + ((d * 8 + 2 * q2) ^ ((g & 3) << 2))) = make_float2(acc[d][2 * r], acc[d][2 * r + 1]);
                 if (q2 == 0) sm_ml[warp * 16 + g + 8 * r] = make_float2(m_i[r], l_i[r]);
             }
             compute_sync();
@@ -360,21 +424,22 @@ attn_shared_kernel(const bf16* __restrict__ q, const bf16* __restrict__ k_pages,
                 const int rho = idx / (HD / 4), x = idx % (HD / 4) * 4;
                 float mm = -INFINITY;
                 #pragma unroll
-                for (int w = 0; w < KQ; w++) mm = fmaxf(mm, sm_ml[w * ROWS + rho].x);
+                for (int w = 0; w < PG; w++) mm = fmaxf(mm, sm_ml[w * ROWS + rho].x);
                 const float m_use = mm == -INFINITY ? 0.f : mm;
                 float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
                 float ll = 0.f;
                 #pragma unroll
-                for (int w = 0; w < KQ; w++) {
+                for (int w = 0; w < PG; w++) {
                     const float2 ml = sm_ml[w * ROWS + rho];
                     const float a = ik_ex2(ml.x - m_use);
-                    const float4 v = *reinterpret_cast<const float4*>(sm_o + (w * ROWS + rho) * LO + x);
+                    const float4 v = *reinterpret_cast<const float4*>(sm_o + (w * ROWS + rho) * HD + (x ^ ((rho & 3) << 2)));
                     sum.x += v.x * a; sum.y += v.y * a; sum.z += v.z * a; sum.w += v.w * a;
                     ll += ml.y * a;
                 }
                 *reinterpret_cast<float4*>(part_o + (slot * ROWS + rho) * HD + x) = sum;
                 if (x == 0) part_ml[slot * ROWS + rho] = make_float2(mm, ll);
             }
+            if (TMA) fence_async();
             compute_sync();
             if (lane == 0) mbar_arrive(&empty[(step - 1) % NS]);
         }
@@ -436,14 +501,22 @@ int launch(const void* q, const void* k_pages, const void* v_pages, void* out, f
            const float* sink_v, int n_pages, int* status, cudaStream_t stream) {
     const size_t slots = (size_t)(c.n_tiles + c.runs) * c.nkv * 16 * RT;
     float2* const part_ml = (float2*)(scratch + slots * HD);
-    const size_t smem = (size_t)NS * STAGE * sizeof(bf16) + (size_t)(c.n_tiles + c.B) * sizeof(int);
+    const size_t smem = FIXED + (size_t)(c.n_tiles + 2 * c.B + c.n_groups + 1) * sizeof(int);
     auto kern = attn_shared_kernel<RT>;
     // one amount whatever the call needs: the attribute belongs to the kernel, and several host threads may launch it
-    const int most = NS * STAGE * (int)sizeof(bf16) + (TILES + SEQS) * (int)sizeof(int);
+    const int most = (int)FIXED + (2 * TILES + 2 * SEQS + 1) * (int)sizeof(int);
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
     if (e != cudaSuccess) return (int)e;
+    CUtensorMap map_k = {}, map_v = {};
+    if (TMA) {
+        const unsigned long long rows = (unsigned long long)n_pages * c.nkv * PAGE;
+        if (rows > 0x7fffffffull) return IK_UNSUPPORTED;
+        int st = ik_make_map(&map_k, k_pages, rows, HD, HD, PAGE);
+        if (st == IK_OK) st = ik_make_map(&map_v, v_pages, rows, HD, HD, PAGE);
+        if (st != IK_OK) return st;
+    }
     IK_RETURN_IF_ERROR(ik_launch(kern, dim3(c.runs, c.nkv), THREADS, smem, stream, (const bf16*)q, (const bf16*)k_pages, (const bf16*)v_pages, scratch, part_ml, c, plan,
-                                 sc_a, sc_b, n_pages, status));
+                                 sc_a, sc_b, n_pages, status, map_k, map_v));
     IK_RETURN_IF_ERROR(ik_launch_family(JOIN_FAMILY, attn_shared_join_kernel, dim3(c.B, c.nh), JT, 0, stream, (const float*)scratch, (const float2*)part_ml, (bf16*)out,
                                         plan, 16 * RT, c.heads, c.nh, c.nkv, sink, sink_v));
     IK_LAUNCH_STATUS();
