@@ -13,10 +13,11 @@
 //
 // A block: one warp brings pages into a ring of shared memory (by TMA with the 128-byte swizzle for head sizes that are multiples of 64, else by cp.async into
 // padded rows: a warp takes 1,700 cycles to issue a page of head size 128 that way, one thread a hundred by TMA), four compute on mma.sync m16n8k16 tiles.
-// A warp owns 16 rows and all 64 keys of a page, with running maximum and sum as floats, base 2.  RT = 1, 2 or 4 warps share a page, one for each 16
-// of a tile's rows, and PG = 4 / RT such groups take turns with the pages: what a page costs besides its products (waits, the maximum's way across lanes) passes
-// on several pages at once.  (With every page's keys shared out to the four warps a page of head size 64 took 2,000 cycles, more than its bytes.)  The groups'
-// results are merged at the end of a tile.  Probabilities are rounded to bfloat16 for the second product, as the other attention kernels do.
+// A warp owns 16 rows and 64 / KQ of a page's keys (RT = 1, 2 or 4 tiles of 16 rows, KQ = 4 / RT), with running maximum and sum as floats, base 2; the
+// warps of equal rows are merged at the end of a tile.  Probabilities are rounded to bfloat16 for the second product, as the other attention kernels do.
+// (A warp to a page, KQ pages at a time, measured 13.5 / 39.2 / 29.1 / 109.6 us where this takes 12.4 / 38.2 / 30.4 / 110.7, with more registers than two blocks leave;
+// shorter runs, 1.5 to 3 to a block's place, 42 to 49 for the second, whether handed out in order or taken by the blocks that finish first: a run costs 2.5 us
+// besides its pages.)
 //
 // Keys behind a sequence's length are masked by position and their values are brought as zeros, so what lies in the unused part of a page never
 // matters.  A page index outside the pool sets *status and is not followed.  A sequence without keys gets zeros.
@@ -134,7 +135,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
 attn_shared_kernel(const bf16* __restrict__ q, const bf16* __restrict__ k_pages, const bf16* __restrict__ v_pages, float* __restrict__ part_o,
                    float2* __restrict__ part_ml, const Call c, const Plan plan, float scale_log2e, float cap_log2e, int n_pages, int* status,
                    const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
-    constexpr int ROWS = 16 * RT, PG = 4 / RT, NB = PAGE / 8, CH = HD / 8;
+    constexpr int ROWS = 16 * RT, KQ = 4 / RT, KEYS = PAGE / KQ, NB = KEYS / 8, CH = HD / 8;
     ik_pdl_wait();
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     bf16* const ring = (bf16*)smem_raw;                              // [NS][keys, values][PAGE][LD]
@@ -252,7 +253,7 @@ attn_shared_kernel(const bf16* __restrict__ q, const bf16* __restrict__ k_pages,
     }
 
     // ---- the computing warps
-    const int g = lane >> 2, q2 = lane & 3, rt = warp % RT, mine = warp / RT;
+    const int g = lane >> 2, q2 = lane & 3, rt = warp % RT, kq = warp / RT;
     int step = 0;
     for (int u = u_first; u < u_end;) {
         while (ends[t] <= u) t++;
@@ -297,18 +298,12 @@ attn_shared_kernel(const bf16* __restrict__ q, const bf16* __restrict__ k_pages,
                 col = o.S;
             }
             const int at = own ? col++ : u - lo, stage = step % NS;          // the page's number in the sequence
-            // every warp sees every page arrive and gives it back, its own behind its work: a barrier's phase that a warp had not seen could be
-            // mistaken for the one before it, or be over before the warp looks
             if (!__all_sync(0xffffffffu, mbar_wait(&full[stage], (step / NS) & 1, &abort_flag, status, IK_WAIT_LIMIT_NS, 42, step))) return;
-            if (step % PG != mine) {
-                if (lane == 0 && u + 1 < stop) mbar_arrive(&empty[stage]);
-                continue;
-            }
             const uint32_t ks_ = smem_u32(ring + stage * STAGE), vs_ = ks_ + HALF * 2;
             if (TMA && own) {                                         // values behind the last key: zeros (by cp.async they come so)
-                const int from = c.kv_lens[member] - at * PAGE;
-                if (from < PAGE) {
-                    for (int i = lane; i < (PAGE - from) * 8; i += 32)
+                const int from = max(c.kv_lens[member] - at * PAGE, kq * KEYS);         // (of this warp's keys)
+                if (from < (kq + 1) * KEYS) {
+                    for (int i = lane; i < ((kq + 1) * KEYS - from) * 8; i += 32)
                         #pragma unroll
                         for (int x = 0; x < HD; x += 64) *reinterpret_cast<uint4*>((unsigned char*)(ring + stage * STAGE + HALF + x * PAGE) + from * 128 + i * 16) = make_uint4(0, 0, 0, 0);
                     __syncwarp();
@@ -325,13 +320,13 @@ attn_shared_kernel(const bf16* __restrict__ q, const bf16* __restrict__ k_pages,
                 #pragma unroll
                 for (int np = 0; np < NB / 2; np++) {
                     uint32_t bfr[4];
-                    ldsm4(bfr, ks_ + piece(np * 16 + (lane & 7) + (lane >> 4) * 8, lane & 7, ks * 2 + ((lane >> 3) & 1)));
+                    ldsm4(bfr, ks_ + piece(kq * KEYS + np * 16 + (lane & 7) + (lane >> 4) * 8, lane & 7, ks * 2 + ((lane >> 3) & 1)));
                     mma(s[2 * np], qf[ks], bfr[0], bfr[1]);
                     mma(s[2 * np + 1], qf[ks], bfr[2], bfr[3]);
                 }
             float mx[2] = {-INFINITY, -INFINITY};
             if (own || ends_early) {
-                const int jbase = at * PAGE + 2 * q2;
+                const int jbase = at * PAGE + kq * KEYS + 2 * q2;
                 #pragma unroll
                 for (int n = 0; n < NB; n++)
                     #pragma unroll
@@ -377,18 +372,41 @@ attn_shared_kernel(const bf16* __restrict__ q, const bf16* __restrict__ k_pages,
                 #pragma unroll
                 for (int d = 0; d < HD / 8; d++) { acc[d][0] *= alpha[0]; acc[d][1] *= alpha[0]; acc[d][2] *= alpha[1]; acc[d][3] *= alpha[1]; }
             }
-            #pragma unroll
-            for (int kk = 0; kk < NB / 2; kk++)
+            auto values = [&](uint32_t (&bfr)[4], int kk, int dp) {
+                ldsm4t(bfr, vs_ + piece(kq * KEYS + kk * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, lane & 7, dp * 2 + (lane >> 4)));
+            };
+            if (!own) {
+                #pragma unroll
+                for (int kk = 0; kk < NB / 2; kk++)
+                    #pragma unroll
+                    for (int dp = 0; dp < HD / 16; dp++) {
+                        uint32_t bfr[4];
+                        values(bfr, kk, dp);
+                        mma(acc[2 * dp], pa[kk], bfr[0], bfr[1]);
+                        mma(acc[2 * dp + 1], pa[kk], bfr[2], bfr[3]);
+                    }
+            } else {
+                // other members' rows have weight 0 on a page that is not theirs, but 0 x inf is not 0: they do not take part
                 #pragma unroll
                 for (int dp = 0; dp < HD / 16; dp++) {
-                    uint32_t bfr[4];
-                    ldsm4t(bfr, vs_ + piece(kk * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, lane & 7, dp * 2 + (lane >> 4)));
-                    mma(acc[2 * dp], pa[kk], bfr[0], bfr[1]);
-                    mma(acc[2 * dp + 1], pa[kk], bfr[2], bfr[3]);
+                    float part[2][4] = {};
+                    #pragma unroll
+                    for (int kk = 0; kk < NB / 2; kk++) {
+                        uint32_t bfr[4];
+                        values(bfr, kk, dp);
+                        mma(part[0], pa[kk], bfr[0], bfr[1]);
+                        mma(part[1], pa[kk], bfr[2], bfr[3]);
+                    }
+                    #pragma unroll
+                    for (int i = 0; i < 2; i++)
+                        #pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            if (seq_of[e >> 1] == member) acc[2 * dp + i][e] += part[i][e];
                 }
+            }
             __syncwarp();
             // the last page of a tile is given back behind the merge below, which uses its space
-            if (lane == 0 && (PG == 1 || u + 1 < stop)) mbar_arrive(&empty[stage]);
+            if (lane == 0 && (KQ == 1 || u + 1 < stop)) mbar_arrive(&empty[stage]);
         }
         const size_t slot = (size_t)(t + run) * c.nkv + kvh;
         #pragma unroll
@@ -396,7 +414,7 @@ attn_shared_kernel(const bf16* __restrict__ q, const bf16* __restrict__ k_pages,
             l_i[r] += __shfl_xor_sync(0xffffffffu, l_i[r], 1);
             l_i[r] += __shfl_xor_sync(0xffffffffu, l_i[r], 2);
         }
-        if (PG == 1) {
+        if (KQ == 1) {
             #pragma unroll
             for (int r = 0; r < 2; r++) {
                 const int rho = rt * 16 + g + 8 * r;
@@ -424,12 +442,12 @@ attn_shared_kernel(const bf16* __restrict__ q, const bf16* __restrict__ k_pages,
                 const int rho = idx / (HD / 4), x = idx % (HD / 4) * 4;
                 float mm = -INFINITY;
                 #pragma unroll
-                for (int w = 0; w < PG; w++) mm = fmaxf(mm, sm_ml[w * ROWS + rho].x);
+                for (int w = 0; w < KQ; w++) mm = fmaxf(mm, sm_ml[w * ROWS + rho].x);
                 const float m_use = mm == -INFINITY ? 0.f : mm;
                 float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
                 float ll = 0.f;
                 #pragma unroll
-                for (int w = 0; w < PG; w++) {
+                for (int w = 0; w < KQ; w++) {
                     const float2 ml = sm_ml[w * ROWS + rho];
                     const float a = ik_ex2(ml.x - m_use);
                     const float4 v = *reinterpret_cast<const float4*>(sm_o + (w * ROWS + rho) * HD + (x ^ ((rho & 3) << 2)));

@@ -364,6 +364,26 @@ def test_a_group_of_everything_and_long_prompts():
     run_shared(32, 8, 128, [8, 8], [130, 33], [130 * 64 + 70 + i for i in range(8)] + [33 * 64 + 1] * 8, seed=10)
 
 
+@pytest.mark.parametrize("hd", [48, 64, 128])
+def test_a_value_that_one_of_a_group_has_stays_with_it(hd):
+    """Infinite and undefined keys and values in a member's own pages: the others' results are those of a call without them, to the last bit."""
+    from ithaca_b200.csrc import attention_bf16
+    g = gen(hd)
+    lens, shared = [200, 260, 130, 64 * 5], 2
+    table, total = layout([4], [shared], lens, 3)
+    q = torch.randn((4, 4 * hd), generator=g).to(torch.bfloat16).to(DEV)
+    k, v = (torch.randn((total, 2, 64, hd), generator=g).to(torch.bfloat16) for _ in range(2))
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    run = lambda k, v: attention_bf16.decode_shared(q, k.to(DEV), v.to(DEV), ints(lens), table.to(DEV), ints([0, 4]), ints([shared] * 4), 1, 4, 2, 3, 4, hd ** -0.5, None)
+    want = run(k, v)
+    for t, x in ((v, math.inf), (v, math.nan), (k, math.nan), (k, -math.inf)):
+        spoilt = t.clone()
+        spoilt[int(table[1, 3]), :, 5] = x
+        got = run(*((k, spoilt) if t is v else (spoilt, v)))
+        assert torch.equal(got[[0, 2, 3]], want[[0, 2, 3]])
+        assert not torch.equal(got[1], want[1])
+
+
 def test_pages_outside_the_pool_are_not_followed():
     from ithaca_b200.csrc import attention_bf16
     k = torch.randn((6, 2, 64, 64), device=DEV).to(torch.bfloat16)
