@@ -39,8 +39,8 @@ constexpr int PAGE = 64;
 constexpr bool TMA = HD % 64 == 0;
 constexpr int LD = TMA ? HD : HD + 8;      // row of a page in shared memory: swizzled blocks of 64 columns, or padded so that consecutive rows fall into different banks
 constexpr int HALF = PAGE * LD, STAGE = 2 * HALF;        // keys (or values) of a page, both, in elements
-constexpr int BLOCKS = HD <= 128 ? 2 : 1;  // blocks of an SM
-constexpr int FIT = 98304 / (STAGE * 2) * (HD <= 128 ? 1 : 2), NS = FIT > 8 ? 8 : FIT < 3 ? 3 : FIT;       // pages of the ring: 96 KB where two blocks share an SM
+constexpr int BLOCKS = HD <= 64 ? 3 : HD <= 128 ? 2 : 1;   // blocks of an SM
+constexpr int FIT = 196608 / BLOCKS / (STAGE * 2), NS = FIT > 8 ? 8 : FIT < 3 ? 3 : FIT;         // pages of the ring: 192 KB an SM
 constexpr int THREADS = 160;               // four computing warps, one that loads
 constexpr size_t RING = (size_t)NS * STAGE * sizeof(bf16), FIXED = RING + 64 * 8 + 2 * NS * 8 + 8;         // bytes of the ring; with results' maxima and sums, barriers, a flag
 constexpr int JOIN_FAMILY = IK_FAMILY_ELEMENTWISE;
@@ -104,8 +104,14 @@ __device__ __forceinline__ TileOf tile_of(const Call& c, const int* starts, cons
     o.S = a < b ? min(max(shared[a], 0), c.table_cols) : 0;
     return o;
 }
+// The order in which a tile's members' own pages come: members whose rows are different warps' take turns, so that several warps have work at a time (where
+// members' rows do not fill 16s evenly: one after the other).  Number i's member, or -1.
+__device__ __forceinline__ int member_at(const Call& c, const TileOf& o, int rt, int i) {
+    const int per_warp = 16 / c.heads, m = 16 % c.heads == 0 ? (i % rt) * per_warp + i / rt : i;
+    return o.first + m < o.last ? o.first + m : -1;
+}
 // pages: how many every sequence has, shared ones included.
-__device__ __forceinline__ int own_pages(const int* pages, const TileOf& o, int seq) { return max(0, pages[seq] - o.S); }
+__device__ __forceinline__ int own_pages(const int* pages, const TileOf& o, int seq) { return seq < 0 ? 0 : max(0, pages[seq] - o.S); }
 __device__ __forceinline__ int pages_in(const int* pages, const TileOf& o) {
     if (o.first >= o.last) return 0;
     int n = o.S;
@@ -208,7 +214,9 @@ attn_shared_kernel(const bf16* __restrict__ q, const bf16* __restrict__ k_pages,
                 int i = u + lane - lo, seq = o.first, col = i;
                 if (i >= o.S) {
                     i -= o.S;
-                    for (int own = own_pages(pages, o, seq); i >= own; own = own_pages(pages, o, seq)) { i -= own; seq++; }
+                    int n = 0;
+                    seq = member_at(c, o, RT, 0);
+                    for (int own = own_pages(pages, o, seq); i >= own; own = own_pages(pages, o, seq)) { i -= own; seq = member_at(c, o, RT, ++n); }
                     col = o.S + i;
                     filled = c.kv_lens[seq] - col * PAGE;
                 }
@@ -278,10 +286,10 @@ attn_shared_kernel(const bf16* __restrict__ q, const bf16* __restrict__ k_pages,
         // rows of a sequence that ends inside the shared pages, against what was asked for, are masked there, too
         const bool ends_early = __any_sync(0xffffffffu, (seq_of[0] >= 0 && pos[0] + 1 < o.S * PAGE) || (seq_of[1] >= 0 && pos[1] + 1 < o.S * PAGE));
         // which own page comes first
-        int member = o.first, col = u - lo;
+        int nth = 0, member = member_at(c, o, RT, 0), col = u - lo;
         if (col >= o.S) {
             int i = col - o.S;
-            for (int own = own_pages(pages, o, member); i >= own; own = own_pages(pages, o, member)) { i -= own; member++; }
+            for (int own = own_pages(pages, o, member); i >= own; own = own_pages(pages, o, member)) { i -= own; member = member_at(c, o, RT, ++nth); }
             col = o.S + i;
         }
         float acc[HD / 8][4], m_i[2] = {-INFINITY, -INFINITY}, l_i[2] = {0.f, 0.f};
@@ -293,12 +301,16 @@ attn_shared_kernel(const bf16* __restrict__ q, const bf16* __restrict__ k_pages,
         for (; u < stop; u++, step++) {
             const bool own = u - lo >= o.S;
             if (own && (u - lo == o.S || col >= pages[member])) {            // the next member that has pages of its own
-                if (u - lo != o.S) member++;
-                while (own_pages(pages, o, member) == 0) member++;
+                if (u - lo != o.S) member = member_at(c, o, RT, ++nth);
+                while (own_pages(pages, o, member) == 0) member = member_at(c, o, RT, ++nth);
                 col = o.S;
             }
             const int at = own ? col++ : u - lo, stage = step % NS;          // the page's number in the sequence
             if (!__all_sync(0xffffffffu, mbar_wait(&full[stage], (step / NS) & 1, &abort_flag, status, IK_WAIT_LIMIT_NS, 42, step))) return;
+            if (own && RT > 1 && !__any_sync(0xffffffffu, seq_of[0] == member || seq_of[1] == member)) {       // another warp's rows
+                if (lane == 0 && (KQ == 1 || u + 1 < stop)) mbar_arrive(&empty[stage]);
+                continue;
+            }
             const uint32_t ks_ = smem_u32(ring + stage * STAGE), vs_ = ks_ + HALF * 2;
             if (TMA && own) {                                         // values behind the last key: zeros (by cp.async they come so)
                 const int from = max(c.kv_lens[member] - at * PAGE, kq * KEYS);         // (of this warp's keys)
