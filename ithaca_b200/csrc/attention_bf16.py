@@ -238,9 +238,26 @@ def shared_module(head_dim: int) -> ctypes.CDLL:
     return ops.timed(m)
 
 
-def sharing_pays(starts, pages, n_pages, n_kv_heads: int, hd: int) -> bool:
-    """Whether a decode step whose sequences share pages so reads them once per group."""
-    return True
+SHARED_SEQS_MOST = SHARED_TILES_MOST = 1024          # what one launch of the kernel for shared pages takes
+
+
+def sharing_pays(n_seqs: int, n_groups: int, max_members: int, shared_bound: int, own_bound: int, n_heads: int, n_kv_heads: int, hd: int) -> bool:
+    """Whether a decode step whose sequences share pages reads them once per group (``decode_shared``), from the sizes that a captured step is kept under.
+
+    It saves (n_seqs - n_groups) readings of the shared pages per kv head, and costs 2 to 4 us more to set up; pages of one's own cost more there the more rows a tile
+    has (all warps pass them, few have work).  us on B200, ``decode`` / ``decode_shared``, pages shared + own: 32 heads of 128 on 8, one group of 4: 8+1 9.2 / 10.4,
+    16+1 11.2 / 10.9, 48+1 16.1 / 11.9; four of 2: 4+1 9.5 / 9.5, 8+1 11.2 / 10.0; four of 8: 2+1 10.8 / 11.6, 4+1 13.7 / 11.6, 2+4 15.3 / 18.2, 4+4 18.2 / 15.9; four of 16:
+    2+1 19.1 / 15.0, 4+4 29.5 / 32.2, 8+4 38.7 / 27.8; sixteen of 4: 1+4 23.8 / 20.8, 48+4 127 / 55; 40 heads on 40, four of 16: 48+1 529 / 62.  32 heads of 64: one
+    group of 4: 16+1 9.1 / 8.9; four of 4: 4+1 8.5 / 9.3, 8+1 10.0 / 9.3."""
+    rows = max_members * (n_heads // n_kv_heads)
+    tall = 16 if rows <= 16 else 32 if rows <= 32 else 64
+    heads = min(n_heads // n_kv_heads, tall)
+    tiles = n_groups * -(-max_members // max(1, min(tall // heads, max_members))) * -(-(n_heads // n_kv_heads) // heads)
+    if n_seqs > SHARED_SEQS_MOST or tiles > SHARED_TILES_MOST:
+        return False
+    least, each = {16: (224, 0.05), 32: (384, 0.4), 64: (512, 0.75)}[tall]
+    saved, own = (n_seqs - n_groups) * shared_bound * n_kv_heads, n_seqs * own_bound * n_kv_heads
+    return saved * (hd + 64) / 192 >= least + each * own
 
 
 def decode_shared(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, kv_lens: torch.Tensor, table: torch.Tensor, starts: torch.Tensor,
@@ -298,7 +315,8 @@ def attend(q, k_pages, v_pages, ctx, table, n_heads: int, scale: float, window: 
         keys = sum(min(e, window + keep + n) if window else e for n, e in zip(ctx.host_n_new, ctx.host_kv_lens))
         rows = hd * 2 + 4 if key_scales is not None else 2 * hd * 2             # bytes of a key (and value) per kv head
         work = (2 * q.numel() * 2 + keys * nkv * rows, 4 * hd * n_heads * pairs)
-    if ctx.is_decode and sharing is not None and not window and key_scales is None and slopes is None:
+    if (ctx.is_decode and sharing is not None and not window and key_scales is None and slopes is None
+            and sharing_pays(ctx.n_seqs, sharing.n_groups, sharing.max_members, sharing.shared_bound, sharing.own_bound, n_heads, nkv, hd)):
         if work is not None:
             once = sum((b - a - 1) * sharing.pages[a] * page_size for a, b in zip(sharing.starts, sharing.starts[1:]))
             work = (work[0] - once * nkv * 4 * hd, work[1])

@@ -107,8 +107,6 @@ class Stepper:
             if (pool.n_shared and grp.window is None and not grp.key_scales and grp.v_head_dim in (None, grp.head_dim) and self.cache.page_size == 64
                     and attention_bf16.supported(grp.head_dim)):
                 found = find_sharing(t, n_pages)
-                if found is not None and not attention_bf16.sharing_pays(found.starts, found.pages, n_pages, grp.n_kv_heads, grp.head_dim):
-                    found = None
             out.append(found)
         return out if any(f is not None for f in out) else []
 

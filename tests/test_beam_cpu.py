@@ -391,3 +391,22 @@ def test_a_step_that_fails_leaves_no_slot_behind():
 
 def test_ranks():
     assert ranked(-6.0, 3, 1.0) == -2.0 and ranked(-6.0, 3, 0.0) == -6.0 and ranked(-6.0, 0, 1.0) == -6.0
+
+
+# heads, kv heads, head size, groups, members, shared, own pages: us of decode, of decode_shared as measured on B200
+MEASURED = [(32, 8, 128, 1, 2, 16, 1, 8.6, 10.0), (32, 8, 128, 1, 4, 8, 1, 9.2, 10.4), (32, 8, 128, 1, 4, 48, 1, 16.1, 11.9), (32, 8, 128, 4, 2, 8, 1, 11.2, 10.0),
+            (32, 8, 128, 4, 8, 2, 1, 10.8, 11.6), (32, 8, 128, 4, 8, 4, 4, 18.2, 15.9), (32, 8, 128, 4, 8, 2, 4, 15.3, 18.2), (32, 8, 128, 4, 16, 2, 1, 19.1, 15.0),
+            (32, 8, 128, 4, 16, 4, 4, 29.5, 32.2), (32, 8, 128, 4, 16, 8, 4, 38.7, 27.8), (32, 8, 128, 16, 4, 48, 4, 127.3, 54.6), (32, 8, 64, 1, 8, 4, 1, 7.6, 9.3),
+            (32, 8, 64, 1, 4, 48, 1, 12.6, 9.7), (32, 8, 64, 4, 16, 8, 1, 21.8, 13.7), (32, 8, 64, 16, 8, 16, 4, 65.6, 30.1), (40, 40, 128, 1, 2, 1, 1, 6.7, 8.6),
+            (40, 40, 128, 1, 4, 8, 1, 17.0, 10.1), (40, 40, 128, 4, 16, 48, 1, 529.3, 61.8), (40, 40, 128, 16, 8, 16, 4, 458.0, 161.5)]
+
+
+@pytest.mark.parametrize("nh,nkv,hd,groups,members,shared,own,apart,together", MEASURED)
+def test_shared_pages_are_read_once_where_that_was_measured_faster(nh, nkv, hd, groups, members, shared, own, apart, together):
+    from ithaca_b200.csrc.attention_bf16 import sharing_pays
+    assert sharing_pays(groups * members, groups, members, shared, own, nh, nkv, hd) == (together < apart)
+
+
+def test_steps_that_are_too_large_for_one_launch_read_their_pages_apart():
+    from ithaca_b200.csrc.attention_bf16 import sharing_pays
+    assert sharing_pays(1024, 64, 16, 50, 1, 32, 8, 128) and not sharing_pays(1040, 65, 16, 50, 1, 32, 8, 128) and not sharing_pays(1024, 512, 2, 50, 1, 320, 1, 128)
