@@ -81,6 +81,32 @@ class PagePool:
         elif self._holders[page] == 1:
             self.n_shared -= 1
 
+    def share_all(self, pages: np.ndarray) -> None:
+        """``share`` of distinct pages at once."""
+        if pages.size == 0:
+            return
+        if pages.min() < 0 or pages.max() >= self.n_pages or (self._holders[pages] == 0).any():
+            for p in pages:                                        # the first that is wrong says what is
+                self._check(int(p))
+                if not self._holders[p]:
+                    raise CacheError(f"page {int(p)} is free and cannot be shared")
+        self._holders[pages] += 1
+        self.n_shared += int((self._holders[pages] == 2).sum())
+
+    def give_back_all(self, pages: np.ndarray) -> None:
+        """``give_back`` of distinct pages at once, in their order."""
+        if pages.size == 0:
+            return
+        if pages.min() < 0 or pages.max() >= self.n_pages or (self._holders[pages] == 0).any():
+            for p in pages:
+                self._check(int(p))
+                if not self._holders[p]:
+                    raise CacheError(f"page {int(p)} is freed twice")
+        self._holders[pages] -= 1
+        left = self._holders[pages]
+        self._free.extend(pages[left == 0].tolist())
+        self.n_shared -= int((left == 1).sum())
+
     def held(self) -> int:
         return int((self._holders > 0).sum())
 
@@ -147,8 +173,7 @@ class SlotTable:
         self._check_slot(slot)
         for g, pool in enumerate(self.pools):
             row = self.tables[g][slot]
-            for i in np.nonzero(row >= 0)[0]:
-                pool.give_back(int(row[i]))
+            pool.give_back_all(row[row >= 0])
             row[:] = -1
         self._in_use[slot] = False
         self.length[slot] = 0
@@ -181,9 +206,7 @@ class SlotTable:
                 for g, pool in enumerate(self.pools):
                     mine, row = self.tables[g][slot], self.tables[g][new]
                     row[:full] = mine[:full]
-                    for p in mine[:full]:
-                        if p >= 0:
-                            pool.share(int(p))
+                    pool.share_all(mine[:full][mine[:full] >= 0])
                     if rows:
                         row[full] = pool.take()
                         copies[g].append((int(mine[full]), int(row[full]), rows))

@@ -221,6 +221,7 @@ def decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, kv_len
 
 
 _shared_modules: Dict[int, ctypes.CDLL] = {}
+_shared_scratch: Dict[tuple, int] = {}         # bytes of scratch by device and sizes
 
 
 def shared_module(head_dim: int) -> ctypes.CDLL:
@@ -284,7 +285,12 @@ def decode_shared(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     if table.dim() != 2 or table.shape[0] != B or table.stride(1) != 1 or n_groups < 1 or not 1 <= max_members <= B:
         raise KernelError("decode_shared: the block table is [sequences, pages], and a group has between one and all of the sequences")
     m = shared_module(hd)
-    need = m.ik_attn_shared_scratch(n_groups, max_members, B, n_heads, nkv)
+    key = (q.get_device(), hd, n_groups, max_members, B, n_heads, nkv)
+    need = _shared_scratch.get(key)
+    if need is None:
+        if len(_shared_scratch) > 4096:
+            _shared_scratch.clear()
+        need = _shared_scratch[key] = m.ik_attn_shared_scratch(n_groups, max_members, B, n_heads, nkv)
     if need < 0:
         raise KernelError(f"decode_shared: {B} sequences in {n_groups} groups of up to {max_members} are more than this kernel takes")
     scratch = torch.empty(need, dtype=torch.uint8, device=q.device)

@@ -22,6 +22,7 @@
 // Keys behind a sequence's length are masked by position and their values are brought as zeros, so what lies in the unused part of a page never
 // matters.  A page index outside the pool sets *status and is not followed.  A sequence without keys gets zeros.
 #include <math.h>
+#include <atomic>
 #define IK_FAMILY 4
 #include "common.cuh"
 #include "tc_common.cuh"
@@ -534,9 +535,18 @@ int launch(const void* q, const void* k_pages, const void* v_pages, void* out, f
     const size_t smem = FIXED + (size_t)(c.n_tiles + 2 * c.B + c.n_groups + 1) * sizeof(int);
     auto kern = attn_shared_kernel<RT>;
     // one amount whatever the call needs: the attribute belongs to the kernel, and several host threads may launch it
+    // (and once a device: asked for at every call it costs the host 1 us)
     const int most = (int)FIXED + (2 * TILES + 2 * SEQS + 1) * (int)sizeof(int);
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+    static std::atomic<unsigned long long> set{0};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return (int)e;
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (dev >= 64 || !(set.load(std::memory_order_acquire) & bit)) {
+        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+        if (e != cudaSuccess) return (int)e;
+        set.fetch_or(bit, std::memory_order_release);
+    }
     CUtensorMap map_k = {}, map_v = {};
     if (TMA) {
         const unsigned long long rows = (unsigned long long)n_pages * c.nkv * PAGE;

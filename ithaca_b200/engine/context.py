@@ -46,6 +46,7 @@ class Sharing:
     pages: List[int]                   # per sequence: pages it shares with its whole group
     shared_bound: int                  # the most pages a group shares
     own_bound: int                     # the most pages a sequence has to itself
+    most: int = 0                      # no group is larger
     starts_dev: Optional[torch.Tensor] = None
     pages_dev: Optional[torch.Tensor] = None
 
@@ -55,7 +56,11 @@ class Sharing:
 
     @property
     def max_members(self) -> int:
-        return max(b - a for a, b in zip(self.starts, self.starts[1:]))
+        return self.most
+
+    def pad(self, n_groups: int) -> None:
+        """Empty groups behind the others, until there are so many."""
+        self.starts += [self.starts[-1]] * (n_groups - self.n_groups)
 
 
 def find_sharing(table: np.ndarray, n_pages: Sequence[int]) -> Optional[Sharing]:
@@ -86,7 +91,7 @@ def find_sharing(table: np.ndarray, n_pages: Sequence[int]) -> Optional[Sharing]
         groups += found[::-1]
     starts = [g[0] for g in groups] + [B]
     pages = [s for (a, s), b in zip(groups, starts[1:]) for _ in range(b - a)]
-    return Sharing(starts, pages, max(pages), max(n - s for n, s in zip(n_pages, pages)))
+    return Sharing(starts, pages, max(pages), max(n - s for n, s in zip(n_pages, pages)), max(b - a for a, b in zip(starts, starts[1:])))
 
 
 def field_offsets(sizes):

@@ -76,10 +76,18 @@ def _bucket(cols: int) -> int:
     return -(-cols // step) * step
 
 
+def _above(n: int) -> int:
+    """The next power of two."""
+    return 1 << max(0, n - 1).bit_length()
+
+
 def _sharing_shape(f: Optional[Sharing]):
-    """What a captured step takes from who shares pages: the number of groups, the largest, and bounds of the pages shared and not (rounded up, so
-    that growing sequences re-capture rarely)."""
-    return None if f is None else (f.n_groups, f.max_members, _bucket(f.shared_bound), _bucket(f.own_bound))
+    """What a captured step takes from who shares pages: the number of groups, the largest, and how many pages are shared and not, all rounded up to
+    powers of two, so that a search whose beams group themselves in another way from step to step replays a handful of graphs.  Groups that do not exist are empty."""
+    if f is None:
+        return None
+    B = f.starts[-1]
+    return min(B, _above(f.n_groups)), min(B, _above(f.max_members)), _above(f.shared_bound), _above(f.own_bound)
 
 
 class GraphDecoder:
@@ -195,6 +203,9 @@ class GraphDecoder:
             sharing = []
             if any(pool.n_shared for pool in table.pools):
                 sharing = st.sharing([t[idx, :cols] for t in table.tables], (lens // page + 1).tolist())
+                for f in sharing:
+                    if f is not None:
+                        f.pad(_sharing_shape(f)[0])
             key = (B, cols) + tuple(_sharing_shape(f) for f in sharing)
             cap = self.graphs.get(key)
             if cap is None:
@@ -270,12 +281,12 @@ class GraphDecoder:
         # room for who shares pages: up to B groups in every key/value group (the buffer may be longer than what it describes)
         room = field_offsets([B, B, B, B + 1, B, B, B] + [B * cols] * n_groups + [B + 1, B] * n_groups)[2]
         buffer = torch.empty(room, dtype=torch.int32, device=st.runtime.device)
-        ctx = st.prepare(slots, tokens, "last", into=buffer, table_cols=cols)
+        ctx = st.prepare(slots, tokens, "last", into=buffer, table_cols=cols, pad=lambda f: f.pad(_sharing_shape(f)[0]))
         sharing = [f for f in ctx.sharing if f is not None]
         offsets, sizes, total = field_offsets([B, B, B, B + 1, B, B, B] + [B * cols] * n_groups + [n for f in sharing for n in (len(f.starts), B)])
         buffer = buffer[:total]
         for f in sharing:                                     # as for the lengths: sizes of grids follow from the shape the graph is kept under
-            _, _, f.shared_bound, f.own_bound = _sharing_shape(f)
+            _, f.most, f.shared_bound, f.own_bound = _sharing_shape(f)
         # the graph is replayed for other lengths: what the kernels choose for it follows from its shape alone, not from which lengths came first
         ctx.kv_len_bound, ctx.replayed = cols * page, True
         torch.cuda.current_stream().synchronize()

@@ -79,8 +79,8 @@ class Stepper:
 
     def prepare(self, slots: Sequence[int], tokens: Sequence[Sequence[int]],
                 want: Union[str, None, Sequence[Sequence[int]]] = "last",
-                into: Optional[torch.Tensor] = None, table_cols: Optional[int] = None) -> StepContext:
-        """Validates, reserves pages and uploads the step's description."""
+                into: Optional[torch.Tensor] = None, table_cols: Optional[int] = None, pad=None) -> StepContext:
+        """Validates, reserves pages and uploads the step's description.  ``pad``: is handed who shares pages before that is uploaded (a captured step keeps room)."""
         want_lists = self._validate(slots, tokens, want)
         n_new = [len(t) for t in tokens]
         self.cache.reserve(slots, n_new)
@@ -93,6 +93,9 @@ class Stepper:
             cols = table_cols
         tables = [self.cache.table.table_rows(g, slots, cols) for g in range(len(self.cache.kv_groups))]
         sharing = self.sharing(tables, [-(-(st + 1) // page) for st in start]) if all(n == 1 for n in n_new) else ()
+        for f in sharing:
+            if pad is not None and f is not None:
+                pad(f)
         return self.builder.build(slots, tokens, start, want_lists, tables, into=into, sharing=sharing)
 
     def sharing(self, tables: Sequence[np.ndarray], n_pages: Sequence[int]) -> List[Optional[Sharing]]:

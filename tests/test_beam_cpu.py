@@ -30,6 +30,21 @@ def test_a_page_is_free_when_its_last_holder_gives_it_back():
             bad()
 
 
+def test_many_pages_at_once():
+    pool = PagePool(6)
+    pages = np.array([pool.take() for _ in range(4)], dtype=np.int32)
+    pool.share_all(pages[1:3])
+    pool.share_all(pages[:0])
+    assert pool.n_shared == 2 and [pool.holders(int(p)) for p in pages] == [1, 2, 2, 1]
+    pool.give_back_all(pages[[3, 1, 0]])
+    assert pool.n_shared == 1 and pool.n_free == 4 and [pool.take(), pool.take()] == [pages[0], pages[3]]        # the last given back comes first
+    for bad in (lambda: pool.share_all(np.array([4])), lambda: pool.give_back_all(np.array([1, 5])), lambda: pool.give_back_all(np.array([6])), lambda: pool.share_all(np.array([-1]))):
+        before = pool._holders.copy(), list(pool._free), pool.n_shared
+        with pytest.raises(CacheError):
+            bad()
+        assert (pool._holders == before[0]).all() and pool._free == before[1] and pool.n_shared == before[2]
+
+
 def table(n_pages=12, slots=6, window=None):
     return SlotTable([KVGroupLayout(2, 16, None, (0, 1)), KVGroupLayout(1, 8, window, (2,))], [n_pages, n_pages], slots, 64)
 
@@ -222,6 +237,16 @@ def test_groups_of_neighbours():
     # the other way round
     s = find_sharing(rows([1, 2, 3, 4, 10], [1, 2, 3, 4, 11], [1, 2, 3, 7, 12], [1, 2, 3, 7, 13]), [5] * 4)
     assert s.starts == [0, 4] and s.pages == [3] * 4 and s.own_bound == 2
+
+
+def test_a_captured_step_keeps_room_for_other_groups():
+    from ithaca_b200.engine.graph import _sharing_shape
+    s = find_sharing(rows([1, 2, 3], [1, 2, 4], [1, 2, 5, 6], [9], [7, 8], [7, 10]), [3, 3, 4, 1, 2, 2])
+    assert _sharing_shape(s) == (4, 4, 2, 2) and _sharing_shape(None) is None
+    s.pad(4)
+    assert s.starts == [0, 3, 4, 6, 6] and s.n_groups == 4 and s.max_members == 3 and _sharing_shape(s) == (4, 4, 2, 2)
+    s = find_sharing(rows([1, 2], [1, 3], [1, 4]), [2, 2, 2])
+    assert _sharing_shape(s) == (1, 3, 1, 1)                                       # never more than there are sequences
 
 
 def test_groups_save_the_most_page_readings():

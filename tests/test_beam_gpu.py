@@ -114,7 +114,7 @@ def test_shared_pages_are_read_once_and_give_the_same(dirs, replayed, monkeypatc
         if n in (0, 1, 40, 69):
             calls.clear()
             got = step(slots, toks)
-            assert calls and all(c[0] == 3 and c[1] == 4 for c in calls) or replayed and not calls
+            assert calls and all(c[0] == (4 if replayed else 3) and c[1] == 4 for c in calls) or replayed and not calls          # a captured step keeps room for a fourth group
             want = np.concatenate([rows(eng, [s], [t]) for s, t in zip(alone, toks)])
             assert off(got, want) <= REL_CUT["bfloat16"]
         else:
