@@ -268,7 +268,7 @@ def decode_shared(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     """Attention of one new token per sequence (``q`` [B, heads * size], bfloat16) over pages of which groups of sequences share the first ones.  ``starts`` int32
     [n_groups + 1]: group g are the sequences starts[g] <= b < starts[g + 1], at most ``max_members`` of them; ``shared`` int32 [B]: how many of sequence b's first pages are
     the same (and full) in all of its group, 0 for a sequence that shares none; a sequence that is in no group gets zeros.  ``shared_bound``, ``own_bound``: about how many pages a group
-    shares and a sequence has of its own at most (the kernel sees the numbers themselves; they are for the caller's choice between this and ``decode``).  At most 1,024 sequences.  All else
+    shares and a sequence has of its own at most (for the caller's choice between this and ``decode``, see ``sharing_pays``; the kernel goes by the numbers themselves).  At most 1,024 sequences.  All else
     as ``decode`` has it, without a window."""
     n_pages, nkv, page_size, hd = k_pages.shape
     B, bf16, i32 = kv_lens.shape[0], torch.bfloat16, torch.int32
@@ -282,6 +282,8 @@ def decode_shared(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     ops._need(table, "table", i32, contiguous=False)
     if starts.numel() != n_groups + 1 or shared.numel() != B:
         raise KernelError(f"decode_shared: {n_groups + 1} starts and {B} numbers of shared pages are needed, found {starts.numel()} and {shared.numel()}")
+    if shared_bound < 0 or own_bound < 0:
+        raise KernelError("decode_shared: the bounds of the pages cannot be negative")
     if table.dim() != 2 or table.shape[0] != B or table.stride(1) != 1 or n_groups < 1 or not 1 <= max_members <= B:
         raise KernelError("decode_shared: the block table is [sequences, pages], and a group has between one and all of the sequences")
     m = shared_module(hd)
@@ -296,6 +298,11 @@ def decode_shared(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
     if out is None:
         out = torch.empty_like(q)
+    else:
+        ops._need(out, "out", bf16)
+        ops._here(out, "out")
+        if out.numel() != q.numel():
+            raise KernelError(f"decode_shared: out has {out.numel()} elements, {q.numel()} are needed")
     ops._work(f"attention decode shared {B}x{n_heads}", *(work or (0, 0)))
     _check(m.ik_attn_shared(_ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(out), _ptr(scratch), _ptr(kv_lens), _ptr(table), table.stride(0), table.shape[1], _ptr(starts),
                             _ptr(shared), n_groups, max_members, B, n_heads, nkv, scale, softcap, ops.sink_flag(sink), _ptr(ops.sink_values(sink, n_heads)), page_size, n_pages,

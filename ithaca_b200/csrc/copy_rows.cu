@@ -6,6 +6,10 @@
 // Sources and destinations of a job are disjoint (the caller checks), so no order among the copies matters.  Bound by memory: every
 // source byte is read once for all its destinations and every destination byte is written once.  Job and move lists travel in the kernel's
 // parameters: no upload, and a captured launch keeps its own.
+//
+// A block moves 8 KB of a segment with four 16-byte loads under way per thread.  us in a replayed graph on B200: six sequences with states of 32 MB each become 24, 126
+// (814 MB, the copy rate); the begun pages of 16 beams in 32 layers, 136 MB in 8,192 segments of 0.25 to 16 KB, 27 (5.1 TB/s); one page of a small model 1.5.  Blocks of 64 to 512
+// threads with 2 to 8 loads: 124-129, 27-37, 1.5-2.2.
 #include <string.h>
 #define IK_FAMILY 1
 #include "common.cuh"

@@ -428,6 +428,82 @@ def test_shared_attention_refuses():
     attention_bf16.decode_shared(**good)
     for bad in (dict(q=q.float()), dict(k_pages=k.float()), dict(v_pages=k[:5]), dict(n_heads=3), dict(q=q[:3]), dict(starts=ints(0, 2, 4)), dict(shared=ints(1, 1)), dict(max_members=0),
                 dict(max_members=5), dict(n_groups=0, starts=ints(0)), dict(table=good["table"][:3]), dict(table=good["table"].long()), dict(kv_lens=good["kv_lens"].cpu()), dict(k_pages=k[:, :, :32], v_pages=k[:, :, :32]),
-                dict(sink=torch.zeros(3, device=DEV)), dict(k_pages=k[..., :24], v_pages=k[..., :24])):
+                dict(sink=torch.zeros(3, device=DEV)), dict(k_pages=k[..., :24], v_pages=k[..., :24]), dict(out=q.float()), dict(out=q[:3]), dict(shared_bound=-1)):
         with pytest.raises(o.KernelError):
             attention_bf16.decode_shared(**{**good, **bad})
+
+
+def test_calls_on_two_streams_at_once():
+    """Each of the three on two streams side by side, many times, with other inputs: none has anything in common with a call beside it."""
+    from ithaca_b200.csrc import attention_bf16
+    g = gen(12)
+    logits = [torch.randn((16, 30011), generator=g).to(DEV) for _ in range(2)]
+    sums = [(torch.rand((4, 4), generator=g) * -5).to(DEV) for _ in range(2)]
+    pages = [torch.randn((3, 40, 2, 64, 32), generator=g).to(DEV) for _ in range(2)]
+    k, v = (torch.randn((60, 2, 64, 128), generator=g).to(torch.bfloat16).to(DEV) for _ in range(2))
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    q = [torch.randn((6, 8 * 128), generator=g).to(torch.bfloat16).to(DEV) for _ in range(2)]
+    table = [ints([[i + 7 * j for i in range(4)] + [30 + 4 * b + i for i in range(4)] for b in range(6)]) for j in range(2)]
+    lens, starts, shared = [ints([400 + 9 * b for b in range(6)]), ints([300, 290, 512, 257, 400, 333])], ints([0, 3, 6]), ints([4] * 6)
+    moves = [([1, 2, 3], [21, 22, 23], [64, 5, 33]), ([7, 7, 9], [30, 31, 32], [12, 12, 64])]
+
+    def run(i):
+        s, b, t = ops().beam_select(logits[i], sums[i], 8)
+        p = pages[i].clone()
+        ops().copy_rows([(p, *moves[i])])
+        a = attention_bf16.decode_shared(q[i], k, v, lens[i], table[i], starts, shared, 2, 3, 4, 4, 8, 0.09, None)
+        return s, b, t, p, a
+
+    want = [[t.clone() for t in run(i)] for i in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(run(i))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for r in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(r, want[i]))
+
+
+def test_two_captured_steps_replayed_in_turn_share_nothing():
+    """Selection and attention captured twice for other inputs; the graphs replayed one after the other, in either order, on two streams."""
+    from ithaca_b200.csrc import attention_bf16
+    g = gen(13)
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    k = torch.randn((40, 2, 64, 64), generator=g).to(torch.bfloat16).to(DEV)
+    cases, graphs = [], []
+    for i in range(2):
+        l, s = torch.randn((8, 5003), generator=g).to(DEV), (torch.rand((2, 4), generator=g) * -4).to(DEV)
+        q = torch.randn((4, 256), generator=g).to(torch.bfloat16).to(DEV)
+        args = (q, k, k, ints([500 - 70 * i] * 4), ints([[j + i for j in range(5)] + [20 + 3 * b + j for j in range(3)] for b in range(4)]), ints([0, 4]), ints([5] * 4), 1, 4, 5, 3, 4, 0.125, None)
+        out, att = torch.zeros((3, 2, 8), dtype=torch.int32, device=DEV), torch.zeros_like(q)
+        want = [t.clone() for t in ops().beam_select(l, s, 8)] + [attention_bf16.decode_shared(*args).clone()]
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            ops().beam_select(l, s, 8, out=out)
+            attention_bf16.decode_shared(*args, out=att)
+        cases.append((l, s, args, out, att, want))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for order in ((0, 1), (1, 0), (0, 0, 1, 1)):
+        for c in cases:
+            c[3].zero_()
+            c[4].zero_()
+        torch.cuda.synchronize()
+        for i in order:
+            with torch.cuda.stream(streams[i]):
+                graphs[i].replay()
+        torch.cuda.synchronize()
+        for l, s, args, out, att, want in cases:
+            assert torch.equal(out[0].view(torch.float32), want[0]) and torch.equal(out[1], want[1]) and torch.equal(out[2], want[2]) and torch.equal(att, want[3])
+
+
+def test_a_vocabulary_of_the_largest_size_and_many_requests():
+    g = gen(14)
+    check_select(torch.randn((2, 1 << 20), generator=g), torch.tensor([[-1.0, -1.5]]), 32)
+    check_select(torch.randn((700 * 3, 37), generator=g), torch.rand((700, 3), generator=g) * -3, 6)
+    with pytest.raises(ops().KernelError):
+        ops().beam_select(torch.zeros((1, (1 << 20) + 1), device=DEV), torch.zeros((1, 1), device=DEV), 2)
