@@ -276,10 +276,13 @@ def decode_shared(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
         raise KernelError("decode_shared: pages of 64 keys and values of one head size, a multiple of 16 up to 256, are supported")
     if n_heads % nkv or q.numel() != B * n_heads * hd:
         raise KernelError(f"decode_shared: queries {tuple(q.shape)} are not {B} times {n_heads} heads of {hd} on {nkv} kv heads")
+    dev = ops._current_device()
     for t, name, dtype in ((q, "q", bf16), (k_pages, "k_pages", bf16), (v_pages, "v_pages", bf16), (kv_lens, "kv_lens", i32), (starts, "starts", i32), (shared, "shared", i32)):
-        ops._need(t, name, dtype)
-        ops._here(t, name)
+        if t.dtype is not dtype or t.get_device() != dev or not t.is_contiguous():       # (-1 on the host)
+            ops._need(t, name, dtype)
+            ops._here(t, name)
     ops._need(table, "table", i32, contiguous=False)
+    ops._here(table, "table")
     if starts.numel() != n_groups + 1 or shared.numel() != B:
         raise KernelError(f"decode_shared: {n_groups + 1} starts and {B} numbers of shared pages are needed, found {starts.numel()} and {shared.numel()}")
     if shared_bound < 0 or own_bound < 0:
@@ -287,7 +290,7 @@ def decode_shared(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     if table.dim() != 2 or table.shape[0] != B or table.stride(1) != 1 or n_groups < 1 or not 1 <= max_members <= B:
         raise KernelError("decode_shared: the block table is [sequences, pages], and a group has between one and all of the sequences")
     m = shared_module(hd)
-    key = (q.get_device(), hd, n_groups, max_members, B, n_heads, nkv)
+    key = (dev, hd, n_groups, max_members, B, n_heads, nkv)
     need = _shared_scratch.get(key)
     if need is None:
         if len(_shared_scratch) > 4096:
@@ -295,7 +298,7 @@ def decode_shared(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
         need = _shared_scratch[key] = m.ik_attn_shared_scratch(n_groups, max_members, B, n_heads, nkv)
     if need < 0:
         raise KernelError(f"decode_shared: {B} sequences in {n_groups} groups of up to {max_members} are more than this kernel takes")
-    scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
+    scratch = q.new_empty((need + 1) // 2)
     if out is None:
         out = torch.empty_like(q)
     else:
@@ -303,10 +306,11 @@ def decode_shared(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
         ops._here(out, "out")
         if out.numel() != q.numel():
             raise KernelError(f"decode_shared: out has {out.numel()} elements, {q.numel()} are needed")
-    ops._work(f"attention decode shared {B}x{n_heads}", *(work or (0, 0)))
-    _check(m.ik_attn_shared(_ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(out), _ptr(scratch), _ptr(kv_lens), _ptr(table), table.stride(0), table.shape[1], _ptr(starts),
-                            _ptr(shared), n_groups, max_members, B, n_heads, nkv, scale, softcap, ops.sink_flag(sink), _ptr(ops.sink_values(sink, n_heads)), page_size, n_pages,
-                            _ptr(status), _stream()), "attention decode (shared pages)", kernels=2)
+    if ops.profiling():
+        ops._work(f"attention decode shared {B}x{n_heads}", *(work or (0, 0)))
+    _check(m.ik_attn_shared(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), scratch.data_ptr(), kv_lens.data_ptr(), table.data_ptr(), table.stride(0),
+                            table.shape[1], starts.data_ptr(), shared.data_ptr(), n_groups, max_members, B, n_heads, nkv, scale, softcap, ops.sink_flag(sink),
+                            _ptr(ops.sink_values(sink, n_heads)) if sink is not False else 0, page_size, n_pages, _ptr(status), _stream()), "attention decode (shared pages)", kernels=2)
     return out
 
 

@@ -1262,8 +1262,12 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n_out: int, out: Opt
     of its softmax probability.  Returns (scores [R, n_out] float32, beams [R, n_out] int32, tokens [R, n_out] int32) of the
     best, descending, equal ones by ascending (beam, token); places without a candidate hold -inf, -1, -1.  Tokens whose logit is -inf or NaN are
     no candidates.  ``out``: int32 [3, R, n_out] to write into (the scores' bits first); the results are views of it."""
-    _need(logits, "logits", torch.float32, contiguous=False)
-    _need(scores, "scores", torch.float32)
+    dev = _current_device()
+    if not (logits.dtype is scores.dtype is torch.float32 and logits.get_device() == scores.get_device() == dev and scores.is_contiguous()):       # (-1 on the host)
+        _need(logits, "logits", torch.float32, contiguous=False)
+        _need(scores, "scores", torch.float32)
+        _here(logits, "logits")
+        _here(scores, "scores")
     if logits.dim() != 2 or scores.dim() != 2 or scores.numel() != logits.shape[0]:
         raise KernelError(f"beam_select: logits {tuple(logits.shape)} and scores {tuple(scores.shape)} do not go together ([R * K, vocab] and [R, K])")
     (R, K), V = scores.shape, logits.shape[1]
@@ -1273,8 +1277,6 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n_out: int, out: Opt
         raise KernelError(f"beam_select: {K} beams, {n_out} results and a vocabulary of {V}: at most {BEAMS_MOST}, 1 to {BEAM_OUT_MOST} and {BEAM_VOCAB_MOST} are supported")
     if logits.stride(1) != 1 and V > 1 or logits.stride(0) < V and R * K > 1:
         raise KernelError("beam_select: the logits' rows must be contiguous and may not overlap")
-    _here(logits, "logits")
-    _here(scores, "scores")
     if out is None:
         out = torch.empty((3, R, n_out), dtype=torch.int32, device=logits.device)
     else:
@@ -1283,9 +1285,10 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n_out: int, out: Opt
         if out.shape != (3, R, n_out):
             raise KernelError(f"beam_select: out must be [3, {R}, {n_out}], found {tuple(out.shape)}")
     need = R * K * -(-V // 1024) * 16
-    scratch = torch.empty(need, dtype=torch.uint8, device=logits.device)
+    scratch = logits.new_empty(need // 4)
     at, part = out.data_ptr(), 4 * R * n_out
-    _work(f"beam select {R}x{K}x{V}", R * K * V * 4 + need)
+    if _profile is not None:
+        _work(f"beam select {R}x{K}x{V}", R * K * V * 4 + need)
     _check(_search_lib().ik_beam_select(logits.data_ptr(), logits.stride(0), scores.data_ptr(), R, K, V, n_out, scratch.data_ptr(), need, at, at + part, at + 2 * part, _stream()),
            "beam_select", kernels=2)
     s, b, v = out.unbind(0)
@@ -1358,7 +1361,8 @@ def copy_rows(jobs) -> None:
             if b[0] < a[1]:
                 raise KernelError("copy_rows: two jobs' tensors overlap")
     j, m = array.array("q", table), array.array("i", moves)
-    _work(f"copy rows {len(moves) // 3} moves in {n_jobs} tensors", nbytes)
+    if _profile is not None:
+        _work(f"copy rows {len(moves) // 3} moves in {n_jobs} tensors", nbytes)
     _check(_search_lib().ik_copy_rows(j.buffer_info()[0], n_jobs, m.buffer_info()[0], len(moves) // 3, _stream()), "copy_rows")
 
 
