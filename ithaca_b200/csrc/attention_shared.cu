@@ -162,6 +162,10 @@ attn_shared_kernel(const bf16* __restrict__ q, const bf16* __restrict__ k_pages,
         for (int s = 0; s < NS; s++) { mbar_init(&full[s], TMA ? 1 : 32); mbar_init(&empty[s], 4); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    if (TMA && tid == 0) {
+        asm volatile("prefetch.tensormap [%0];" :: "l"(&map_k) : "memory");
+        asm volatile("prefetch.tensormap [%0];" :: "l"(&map_v) : "memory");
+    }
     // the block tables, on their way to L2 while the plan is made (all blocks together)
     for (long long i = (long long)(blockIdx.y * gridDim.x + blockIdx.x) * THREADS + tid; i * 32 < (long long)c.B * c.table_stride; i += (long long)gridDim.x * gridDim.y * THREADS)
         asm volatile("prefetch.global.L2 [%0];" :: "l"(c.table + min(i * 32, (long long)(c.B - 1) * c.table_stride + c.table_cols - 1)));

@@ -17,7 +17,7 @@
 //
 // Scores are formed and compared in 64 bits (two beams' candidates may be closer than a float of their size can tell) and rounded once;
 // exponentials are floats, summed in float within a tile and in 64 bits beyond.  A logit of -inf or NaN is no candidate; neither is any of a beam
-// whose sum is -inf or NaN.  Where a row has logits of +inf, they share the probability.  Places without a candidate: score -inf, beam and token -1.
+// whose sum is -inf or NaN, nor one whose score is below what a float holds.  Where a row has logits of +inf, they share the probability.  Places without a candidate: score -inf, beam and token -1.
 #include <math.h>
 #define IK_FAMILY 16
 #include "common.cuh"
@@ -187,7 +187,7 @@ __device__ __forceinline__ double score_of(const Beam& b, float l) {
 }
 __device__ __forceinline__ Cand cand_of(const Beam& b, float l, uint32_t at) {
     const double s = score_of(b, l);
-    return pick(s > -INFINITY, none(), Cand{order_key(s), at});
+    return pick((float)s > -INFINITY, none(), Cand{order_key(s), at});
 }
 
 template <bool VEC>
@@ -197,10 +197,11 @@ beam_merge_kernel(const float* __restrict__ logits, long long ldl, const Tile* _
     __shared__ Beam beams[BEAMS];
     __shared__ float sorted[2 * MW][32];                               // lists of the merge's levels, one behind the other
     __shared__ Cand cand[PICKS * OUT], picked[OUT * 32];               // candidates; tiles by their maxima
-    __shared__ int picked_tile[OUT * 32], chosen[PICKS];
+    __shared__ int picked_tile[OUT * 32], chosen[PICKS], order[OUT];
     __shared__ int n_picked, n_cand;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = blockIdx.x, total = K * tiles;
     if (tid == 0) n_picked = n_cand = 0;
+    if (tid < OUT) order[tid] = -1;
     ik_pdl_wait();
     IK_AFTER_WAIT(tile_of);
     IK_AFTER_WAIT(sums);
@@ -337,14 +338,14 @@ beam_merge_kernel(const float* __restrict__ logits, long long ldl, const Tile* _
     }
     __syncthreads();
     const int c = n_cand;
-    for (int i = warp; i < c; i += MW) {
+    for (int i = warp; i < c; i += MW) {                               // (what turned out to be no candidate stands behind all that are)
         const int rank = rank_of(cand, c, i, lane);
-        if (lane == 0 && rank < n) chosen[rank] = i;
+        if (lane == 0 && rank < n) order[rank] = i;
     }
     __syncthreads();
     if (tid < n) {
-        const bool is = tid < c;
-        const Cand me = is ? cand[chosen[tid]] : none();
+        const Cand me = order[tid] < 0 ? none() : cand[order[tid]];
+        const bool is = me.s != 0ull;
         const int b = (int)(me.at / (uint32_t)V);
         out_s[r * n + tid] = is ? (float)order_value(me.s) : -INFINITY;
         out_b[r * n + tid] = is ? b : -1;

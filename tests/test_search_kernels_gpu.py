@@ -121,6 +121,19 @@ def test_equal_candidates_come_by_beam_and_token():
     assert b[0].tolist() == [0] * 20 and v[0].tolist() == list(range(20))
 
 
+def test_scores_below_the_range_of_a_float_are_no_candidates():
+    """Tokens masked by the type's lowest value, of beams whose sums are such values already."""
+    l = torch.full((4, 2000), LOWEST)
+    l[0, 5] = l[1, 7] = l[2, 1999] = 1.0
+    s, b, v = (t.cpu() for t in ops().beam_select(l.to(DEV), torch.tensor([[-1.0, -2.0], [LOWEST, LOWEST]], device=DEV), 4))
+    # beam 0's and 1's own tokens, then beam 0's first masked ones; the second request: one token costs nothing, all others two lowest values
+    assert b.tolist() == [[0, 1, 0, 0], [0, 1, 1, 1]] and v.tolist() == [[5, 7, 0, 1], [1999, 0, 1, 2]]
+    # (a row of nothing but the lowest value is an even distribution)
+    assert s[0].tolist() == pytest.approx([-1.0, -2.0, LOWEST, LOWEST]) and s[1].tolist() == pytest.approx([LOWEST] * 4)
+    s, b, v = (t.cpu() for t in ops().beam_select(l[:3].to(DEV), torch.tensor([[LOWEST, LOWEST, LOWEST]], device=DEV), 5))
+    assert b.tolist() == [[0, 1, 2, -1, -1]] and v.tolist() == [[5, 7, 1999, -1, -1]] and s[0, 3:].tolist() == [-math.inf] * 2
+
+
 def test_dead_beams_are_left_alone():
     g = gen(3)
     l = torch.randn((8, 501), generator=g)
