@@ -268,6 +268,7 @@ attn_shared_kernel(const bf16* __restrict__ q, const bf16* __restrict__ k_pages,
     // ---- the computing warps
     const int g = lane >> 2, q2 = lane & 3, rt = warp % RT, kq = warp / RT;
     int step = 0;
+    bool alive = true;                                               // behind a wait that ran out a warp does no more work, but meets the others where they wait for it
     for (int u = u_first; u < u_end;) {
         while (ends[t] <= u) t++;
         const int lo = t ? ends[t - 1] : 0, stop = min(ends[t], u_end);
@@ -311,7 +312,8 @@ attn_shared_kernel(const bf16* __restrict__ q, const bf16* __restrict__ k_pages,
                 col = o.S;
             }
             const int at = own ? col++ : u - lo, stage = step % NS;          // the page's number in the sequence
-            if (!__all_sync(0xffffffffu, mbar_wait(&full[stage], (step / NS) & 1, &abort_flag, status, IK_WAIT_LIMIT_NS, 42, step))) return;
+            alive = alive && __all_sync(0xffffffffu, mbar_wait(&full[stage], (step / NS) & 1, &abort_flag, status, IK_WAIT_LIMIT_NS, 42, step));
+            if (!alive) continue;
             if (own && RT > 1 && !__any_sync(0xffffffffu, seq_of[0] == member || seq_of[1] == member)) {       // another warp's rows
                 if (lane == 0 && (KQ == 1 || u + 1 < stop)) mbar_arrive(&empty[stage]);
                 continue;
@@ -503,7 +505,8 @@ attn_shared_join_kernel(const float* __restrict__ part_o, const float2* __restri
     for (int j = over.x + grp; j <= over.y; j += JG) {
         const size_t at = ((size_t)(t + j) * nkv + kvh) * rows + row;
         const float2 ml = part_ml[at];
-        const float4 v = *reinterpret_cast<const float4*>(part_o + at * HD + x * 4);
+        float4 v = *reinterpret_cast<const float4*>(part_o + at * HD + x * 4);
+        if (ml.y == 0.f) v = make_float4(0.f, 0.f, 0.f, 0.f);          // a sequence without keys takes nothing from its neighbours' pages, be they infinite
         const float m_new = fmaxf(m, ml.x), m_use = m_new == -INFINITY ? 0.f : m_new, a = ik_ex2(m - m_use), w = ik_ex2(ml.x - m_use);
         sum = make_float4(sum.x * a + v.x * w, sum.y * a + v.y * w, sum.z * a + v.z * w, sum.w * a + v.w * w);
         l = l * a + ml.y * w;

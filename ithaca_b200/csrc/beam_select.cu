@@ -139,10 +139,6 @@ __device__ __forceinline__ float shfl_xor(float c, int m) { return __shfl_xor_sy
 __device__ __forceinline__ float exchange(bool front, float mine, float other) { return front ? fmaxf(mine, other) : fminf(mine, other); }
 __device__ __forceinline__ Cand exchange(bool front, const Cand& mine, const Cand& other) { return pick(front == ahead(other, mine), mine, other); }
 __device__ __forceinline__ float better(float a, float b) { return fmaxf(a, b); }
-__device__ __forceinline__ uint32_t order_key(float v) {               // orders like the value; more than 0
-    const uint32_t b = __float_as_uint(v);
-    return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-}
 
 // A warp's 32 candidates (or floats) in order, lane 0 the best: bitonic.
 template <typename T>
@@ -324,15 +320,22 @@ beam_merge_kernel(const float* __restrict__ logits, long long ldl, const Tile* _
             base += before - __popc(in);
             for (; in; in &= in - 1) put(base++, lo + place_in<VEC>(__ffs(in) - 1, lane));
         } else {
-            for (int j = 0; j < n; j++) {                              // the largest logit that is left, the first of equals
-                float top = -INFINITY;
-                int from = -1;
+            unsigned long long key[PER];                               // 0: no candidate
+            #pragma unroll
+            for (int e = 0; e < PER; e++) key[e] = in >> e & 1 ? cand_of(beam, v[e], 0).s : 0ull;
+            #pragma unroll 1
+            for (int j = 0; j < n; j++) {                              // the best that is left.  (By its score: of large sums several logits give the same)
+                Cand top = none();
+                int from = 0;
                 #pragma unroll
-                for (int e = PER - 1; e >= 0; e--)
-                    if ((in >> e & 1) && v[e] >= top) { top = v[e]; from = e; }
-                const uint32_t key = from < 0 ? 0u : order_key(top), most = __reduce_max_sync(0xffffffffu, key);
-                const int at = key == most ? place_in<VEC>(from, lane) : TILE, first = __reduce_min_sync(0xffffffffu, at);
-                if (at == first) { put(base + j, lo + at); in &= ~(1u << from); }
+                for (int e = PER - 1; e >= 0; e--)                     // (a lane's places ascend)
+                    if ((in >> e & 1) && key[e] && key[e] >= top.s) { top.s = key[e]; from = e; }
+                if (top.s) top.at = (uint32_t)b * (uint32_t)V + (uint32_t)(lo + place_in<VEC>(from, lane));
+                Cand most = top;
+                #pragma unroll
+                for (int o = 16; o > 0; o >>= 1) most = better(most, shfl_xor(most, o));
+                if (lane == 0) cand[base + j] = most;
+                if (top.at == most.at) in &= ~(1u << from);            // (nothing is left where that is several lanes)
             }
         }
     }
@@ -347,9 +350,10 @@ beam_merge_kernel(const float* __restrict__ logits, long long ldl, const Tile* _
         const Cand me = order[tid] < 0 ? none() : cand[order[tid]];
         const bool is = me.s != 0ull;
         const int b = (int)(me.at / (uint32_t)V);
-        out_s[r * n + tid] = is ? (float)order_value(me.s) : -INFINITY;
-        out_b[r * n + tid] = is ? b : -1;
-        out_v[r * n + tid] = is ? (int)(me.at - (uint32_t)b * (uint32_t)V) : -1;
+        const size_t to = (size_t)r * n + tid;
+        out_s[to] = is ? (float)order_value(me.s) : -INFINITY;
+        out_b[to] = is ? b : -1;
+        out_v[to] = is ? (int)(me.at - (uint32_t)b * (uint32_t)V) : -1;
     }
 }
 

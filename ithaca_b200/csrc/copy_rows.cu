@@ -88,15 +88,25 @@ __global__ void __launch_bounds__(CT) copy_rows_kernel(const __grid_constant__ W
 // sizes in bytes).  moves: per move src, dst, positions.  The lists are read before the call returns.
 IK_EXPORT int ik_copy_rows(const long long* jobs, int n_jobs, const int* moves, int n_moves, cudaStream_t stream) {
     if (n_jobs < 0 || n_moves < 0) return IK_BAD_ARGUMENT;
+    constexpr long long BLOCKS = 0x7fffffff;                             // of a launch
+    auto width_of = [](const long long* a) {
+        const long long all = a[0] | a[2] | a[4] | a[6];
+        return all % 16 == 0 ? 16 : (all | a[7]) % 4 == 0 ? 4 : 2;
+    };
+    auto chunks_of = [&](const long long* a, long long part) { const long long piece = (long long)CT * CU * width_of(a); return (part + piece - 1) / piece; };
     for (int j = 0; j < n_jobs; j++) {
         const long long* a = jobs + 10 * j;
         if (!a[0] || a[1] <= 0 || a[1] > 0x7fffffff || a[3] <= 0 || a[5] <= 0 || a[5] > 0x7fffffff || a[7] <= 0 || (a[7] & 1) || (a[0] & 1) || (a[2] & 1) || (a[4] & 1) || (a[6] & 1) ||
             a[8] < 0 || a[9] < 0 || a[8] + a[9] > n_moves)
             return IK_BAD_ARGUMENT;
+        int longest = 0;
         for (long long i = a[8]; i < a[8] + a[9]; i++) {
             const int* m = moves + 3 * i;
             if (m[0] < 0 || m[0] >= a[3] || m[1] < 0 || m[1] >= a[3] || m[0] == m[1] || m[2] < 0) return IK_BAD_ARGUMENT;
+            if (m[2] > longest) longest = m[2];
         }
+        // a launch takes all entries and segments of a job, so that many blocks have to fit: told here, before anything is copied
+        if ((double)chunks_of(a, longest * a[7]) * (double)a[5] * (double)a[1] * (double)(a[9] < MOVES ? a[9] : MOVES) > (double)BLOCKS) return IK_UNSUPPORTED;
     }
     Work w;
     w.n_jobs = 0;
@@ -119,9 +129,9 @@ IK_EXPORT int ik_copy_rows(const long long* jobs, int n_jobs, const int* moves, 
             if (w.n_jobs == JOBS || used == MOVES || used_dst + FAN > DSTS) { int st = flush(); if (st) return st; }
             Job& job = w.jobs[w.n_jobs];
             job.base = (char*)a[0]; job.entries = (int)a[1]; job.entry_stride = a[2]; job.row_stride = a[4]; job.segs = (int)a[5]; job.seg_stride = a[6];
-            const long long all = a[0] | a[2] | a[4] | a[6];
-            job.width = all % 16 == 0 ? 16 : (all | a[7]) % 4 == 0 ? 4 : 2;
+            job.width = width_of(a);
             job.first_move = used; job.first_block = blocks;
+            const long long from = i;
             long long most = 0;
             while (i < end && used < MOVES && used_dst + FAN <= DSTS) {
                 Move& m = w.moves[used];
@@ -133,16 +143,13 @@ IK_EXPORT int ik_copy_rows(const long long* jobs, int n_jobs, const int* moves, 
                 used++;
             }
             job.n_moves = used - job.first_move;
-            const long long piece = (long long)CT * CU * job.width;
-            const long long chunks = (most + piece - 1) / piece;
-            if (chunks > 0x7fffffff) return IK_UNSUPPORTED;
-            job.chunks = (int)chunks;
-            const long long more = chunks * job.segs * job.n_moves * job.entries;
-            if (more > 0x7fffffff) return IK_UNSUPPORTED;
-            if (more == 0) { used = job.first_move; used_dst = used ? w.moves[used - 1].first_dst + w.moves[used - 1].n_dst : 0; continue; }
-            if (blocks + more > 0x7fffffff) {                            // this job goes into a launch of its own
-                used = job.first_move; used_dst = used ? w.moves[used - 1].first_dst + w.moves[used - 1].n_dst : 0;
-                return IK_UNSUPPORTED;
+            job.chunks = (int)chunks_of(a, most);
+            const long long more = (long long)job.chunks * job.segs * job.n_moves * job.entries;
+            if (more == 0 || blocks + more > BLOCKS) {                   // nothing to copy, or this job goes into the next launch
+                used = job.first_move;
+                used_dst = used ? w.moves[used - 1].first_dst + w.moves[used - 1].n_dst : 0;
+                if (more) { i = from; int st = flush(); if (st) return st; }
+                continue;
             }
             blocks += more;
             w.n_jobs++;

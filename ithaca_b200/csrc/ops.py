@@ -1275,6 +1275,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n_out: int, out: Opt
         raise KernelError("beam_select: there is nothing to choose from")
     if K > BEAMS_MOST or not 1 <= n_out <= BEAM_OUT_MOST or V > BEAM_VOCAB_MOST:
         raise KernelError(f"beam_select: {K} beams, {n_out} results and a vocabulary of {V}: at most {BEAMS_MOST}, 1 to {BEAM_OUT_MOST} and {BEAM_VOCAB_MOST} are supported")
+    if R * K > 0x3fffffff:
+        raise KernelError(f"beam_select: {R} requests are too many")
     if logits.stride(1) != 1 and V > 1 or logits.stride(0) < V and R * K > 1:
         raise KernelError("beam_select: the logits' rows must be contiguous and may not overlap")
     if out is None:
@@ -1284,6 +1286,9 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n_out: int, out: Opt
         _here(out, "out")
         if out.shape != (3, R, n_out):
             raise KernelError(f"beam_select: out must be [3, {R}, {n_out}], found {tuple(out.shape)}")
+        lo, hi = out.data_ptr(), out.data_ptr() + 12 * R * n_out
+        if lo < scores.data_ptr() + 4 * R * K and scores.data_ptr() < hi or lo < logits.data_ptr() + 4 * ((R * K - 1) * logits.stride(0) + V) and logits.data_ptr() < hi:
+            raise KernelError("beam_select: out may not overlap the logits or the scores")
     need = R * K * -(-V // 1024) * 16
     scratch = logits.new_empty(need // 4)
     at, part = out.data_ptr(), 4 * R * n_out

@@ -134,6 +134,17 @@ def test_scores_below_the_range_of_a_float_are_no_candidates():
     assert b.tolist() == [[0, 1, 2, -1, -1]] and v.tolist() == [[5, 7, 1999, -1, -1]] and s[0, 3:].tolist() == [-math.inf] * 2
 
 
+@pytest.mark.parametrize("V", [1500, 1501, 5000])
+def test_sums_beside_which_logits_do_not_count(V):
+    """Beams that all have the type's lowest value, or something as large, as their sum: in 64 bits every score is the same, and the first tokens are chosen."""
+    l = torch.randn((2, V), generator=gen(V))
+    for c in (LOWEST, -1e30):
+        s, b, v = (t.cpu() for t in ops().beam_select(l.to(DEV), torch.full((1, 2), c, device=DEV), 8))
+        assert s[0].tolist() == pytest.approx([c] * 8) and b[0].tolist() == [0] * 8 and v[0].tolist() == list(range(8))
+    s, b, v = (t.cpu() for t in ops().beam_select(l.to(DEV), torch.tensor([[LOWEST, -1.0]], device=DEV), 8))
+    assert b[0].tolist() == [1] * 8 and v[0].tolist() == torch.sort(l[1], descending=True).indices[:8].tolist()
+
+
 def test_dead_beams_are_left_alone():
     g = gen(3)
     l = torch.randn((8, 501), generator=g)
@@ -193,6 +204,12 @@ def test_select_refuses():
                 lambda: o.beam_select(l[:1].expand(4, 10), s, 2)):
         with pytest.raises(o.KernelError):
             bad()
+    both = torch.zeros(200, device=DEV)                             # results may not be written where the inputs are read
+    for logits, scores, at in ((both[:40].view(4, 10), s, 30), (l, both[40:44].view(2, 2), 36), (l, both[40:44].view(2, 2), 40)):
+        out = both[at:at + 12].view(torch.int32).view(3, 2, 2)
+        with pytest.raises(o.KernelError, match="overlap"):
+            o.beam_select(logits, scores, 2, out=out)
+    o.beam_select(both[:40].view(4, 10), both[40:44].view(2, 2), 2, out=both[44:56].view(torch.int32).view(3, 2, 2))
 
 
 # -- copies ----------------------------------------------------------------------------------------------------------------
@@ -395,6 +412,23 @@ def test_a_value_that_one_of_a_group_has_stays_with_it(hd):
         got = run(*((k, spoilt) if t is v else (spoilt, v)))
         assert torch.equal(got[[0, 2, 3]], want[[0, 2, 3]])
         assert not torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("sink", [False, True])
+@pytest.mark.parametrize("hd", [64, 48])
+def test_a_sequence_without_keys_takes_nothing_from_its_neighbours(hd, sink):
+    """A place of a padded batch stands in a group whose shared pages hold infinite values: zeros."""
+    from ithaca_b200.csrc import attention_bf16
+    g = gen(hd)
+    lens = [200, 0, 130]
+    table, total = layout([3], [2], [200, 130, 130], 3)
+    q = torch.randn((3, 4 * hd), generator=g).to(torch.bfloat16).to(DEV)
+    k, v = (torch.randn((total, 2, 64, hd), generator=g).to(torch.bfloat16) for _ in range(2))
+    v[int(table[0, 0]), :, 5, 3], v[int(table[0, 1]), :, 7, 4] = math.inf, math.nan
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    got = attention_bf16.decode_shared(q, k.to(DEV), v.to(DEV), ints(lens), table.to(DEV), ints([0, 3]), ints([2, 2, 2]), 1, 3, 2, 2, 4, hd ** -0.5, None, sink=sink).view(3, 4, hd)
+    assert (got[1] == 0).all() and (got[[0, 2]][..., 3] == math.inf).all() and torch.isnan(got[[0, 2]][..., 4]).all()
+    assert torch.isfinite(got[[0, 2]][..., 5:]).all()
 
 
 def test_pages_outside_the_pool_are_not_followed():
