@@ -161,7 +161,13 @@ class SequenceCache:
         states are copied, all layers and slots in one launch.  CacheFull if slots or pages do not suffice; nothing has changed then."""
         made, copies = self.table.fork(wanted)
         src = [slot for (slot, _), new in zip(wanted, made) for _ in new]
-        self._copy(copies, src, [s for new in made for s in new])
+        to = [s for new in made for s in new]
+        try:
+            self._copy(copies, src, to)
+        except Exception:
+            for s in to:
+                self.table.free_slot(s)
+            raise
         return made
 
     def _copy(self, pages: Sequence[Sequence[Tuple[int, int, int]]], from_slots: Sequence[int], to_slots: Sequence[int]) -> None:
@@ -177,7 +183,8 @@ class SequenceCache:
             jobs += [(t, from_slots, to_slots, None) for t in self.state]
         if jobs:
             from ..csrc import ops
-            ops.copy_rows(jobs)
+            with torch.cuda.device(self.device):
+                ops.copy_rows(jobs)
 
     def length(self, slot: int) -> int:
         self.table._check_slot(slot)

@@ -37,8 +37,8 @@ class BeamOptions:
             raise ValueError(f"beams must be between 1 and {BEAMS_MOST}, found {self.beams}")
         if not 1 <= self.n_best <= self.beams:
             raise ValueError(f"n_best must be between 1 and the number of beams, found {self.n_best}")
-        if not self.length_penalty >= 0:
-            raise ValueError(f"length_penalty must be >= 0, found {self.length_penalty}")
+        if not 0 <= self.length_penalty <= 32:                # (a length to a higher power may pass the largest float)
+            raise ValueError(f"length_penalty must be between 0 and 32, found {self.length_penalty}")
 
 
 @dataclass

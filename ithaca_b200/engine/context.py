@@ -8,7 +8,7 @@ the sequence's length before the step plus k.
 from __future__ import annotations
 
 from dataclasses import dataclass, field
-from typing import List, Optional, Sequence
+from typing import List, Optional, Sequence, Tuple
 
 import numpy as np
 import torch
@@ -70,28 +70,52 @@ def find_sharing(table: np.ndarray, n_pages: Sequence[int]) -> Optional[Sharing]
     B = table.shape[0]
     if B < 2:
         return None
-    common = np.cumprod((table[1:] == table[:-1]) & (table[1:] >= 0), axis=1).sum(axis=1)
+    other = (table[1:] != table[:-1]) | (table[1:] < 0)
+    first = other.argmax(axis=1)                                   # 0 where there is none, too
+    common = np.where(other[np.arange(B - 1), first], first, table.shape[1])
     if not common.any():
         return None
-
-    # best[j]: the most that rows .. j - 1 save; a group of rows i .. j - 1 adds (j - 1 - i) * min(common[i:j - 1]).  Runs without a common page are told apart first
-    groups = []                                                    # (first row, pages shared)
-    edges = np.concatenate(([0], np.flatnonzero(common == 0) + 1, [B]))
-    for lo, hi in zip(edges[:-1].tolist(), edges[1:].tolist()):
-        best, cuts = np.zeros(hi - lo + 1, dtype=np.int64), [(0, 0)] * (hi - lo + 1)
-        for j in range(1, hi - lo + 1):
-            least = np.concatenate((np.minimum.accumulate(common[lo:lo + j - 1][::-1])[::-1], [0]))       # of rows i .. j - 1, for every i
-            gain = best[:j] + np.arange(j - 1, -1, -1) * least
-            i = int(gain.argmax())                                 # of equal ways the larger group
-            best[j], cuts[j] = gain[i], (i, int(least[i]))
-        at, found = hi - lo, []
-        while at > 0:
-            at, least_here = cuts[at]
-            found.append((lo + at, least_here))
-        groups += found[::-1]
-    starts = [g[0] for g in groups] + [B]
-    pages = [s for (a, s), b in zip(groups, starts[1:]) for _ in range(b - a)]
+    starts, pages, lo, common = [], [], 0, common.tolist() + [0]
+    for hi, c in enumerate(common, 1):
+        if c:
+            continue
+        # rows lo .. hi - 1 are a run whose neighbours all have pages in common
+        for a, b, s in _cut_run(common[lo:hi - 1]):
+            starts.append(lo + a)
+            pages += [s] * (b - a)
+        lo = hi
+    starts.append(B)
     return Sharing(starts, pages, max(pages), max(n - s for n, s in zip(n_pages, pages)), max(b - a for a, b in zip(starts, starts[1:])))
+
+
+def _cut_run(c: List[int]) -> List[Tuple[int, int, int]]:
+    """``c``: the pages that each of a run's len(c) + 1 rows has in common with the next.  The groups (first row, row behind the last, pages in common) that save
+    the most; of equal ways the larger group."""
+    m = len(c) + 1
+    if len(set(c)) < 2:
+        return [(0, m, c[0] if c else 0)]
+    # What a cut within a stretch of equal numbers saves is linear in where it lies: only its two ends need looking at
+    at = [0] + [j for j in range(1, m) if j == 1 or j == m - 1 or c[j - 1] != c[j - 2] or c[j - 1] != c[j]] + [m]
+    least = [min(c[i:j]) if j < m else 0 for i, j in zip(at, at[1:])]                   # of the rows between two of them, with the cut's own
+    best, cuts = [0], [(0, 0)]
+    for y in range(1, len(at)):
+        most, cut, low = best[y - 1], (y - 1, 0), 0
+        if at[y] - at[y - 1] > 1:
+            low = min(c[at[y - 1]:at[y] - 1])
+            most, cut = most + (at[y] - at[y - 1] - 1) * low, (y - 1, low)
+        for x in range(y - 2, -1, -1):
+            low = min(low or least[x], least[x])
+            gain = best[x] + (at[y] - at[x] - 1) * low
+            if gain >= most:
+                most, cut = gain, (x, low)
+        best.append(most)
+        cuts.append(cut)
+    groups, y = [], len(at) - 1
+    while y:
+        x, low = cuts[y]
+        groups.append((at[x], at[y], low))
+        y = x
+    return groups[::-1]
 
 
 def field_offsets(sizes):

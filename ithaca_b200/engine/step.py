@@ -110,6 +110,10 @@ class Stepper:
             if (pool.n_shared and grp.window is None and not grp.key_scales and grp.v_head_dim in (None, grp.head_dim) and self.cache.page_size == 64
                     and attention_bf16.supported(grp.head_dim)):
                 found = find_sharing(t, n_pages)
+                # too little for any number of heads, and a captured step rounds the shared pages up to less than twice as many: the step is as any other
+                if found is not None and not attention_bf16.sharing_pays(len(n_pages), found.n_groups, found.max_members, 2 * found.shared_bound, 0,
+                                                                         grp.n_kv_heads, grp.n_kv_heads, grp.head_dim):
+                    found = None
             out.append(found)
         return out if any(f is not None for f in out) else []
 

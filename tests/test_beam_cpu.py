@@ -1,4 +1,5 @@
 """Forked slots and shared pages in the cache's books, who shares pages in a step, and the search's decisions: no device."""
+import array
 import itertools
 import math
 import random
@@ -210,6 +211,21 @@ def test_the_cache_forks_without_a_device():
         c.truncate(1, 10)
 
 
+def test_a_fork_whose_copies_fail_changes_nothing(monkeypatch):
+    c = SequenceCache({0: [KVRequest(2, 16)]}, max_tokens=640, max_slots=4, device=None)
+    a = c.alloc_slot()
+    c.reserve([a], [70])
+    c.commit([a], [70])
+    free = [p.n_free for p in c.table.pools]
+    def fail(*a):
+        raise KernelError("lost")
+    monkeypatch.setattr(c, "_copy", fail)
+    with pytest.raises(KernelError, match="lost"):
+        c.fork([(a, 2)])
+    assert c.table.n_slots_in_use() == 1 and [p.n_free for p in c.table.pools] == free and c.table.pools[0].n_shared == 0
+    c.table.check_consistent()
+
+
 def test_lists_of_moves_are_checked():
     assert copy_moves([1, 1], (2, 3), [4, 0], 4, 64) == [1, 2, 4, 1, 3, 0] and copy_moves([1, 0], [2, 3], None, 4, 1) == [1, 2, 1, 0, 3, 1]
     assert copy_moves([], [], None, 4, 1) == []
@@ -217,6 +233,18 @@ def test_lists_of_moves_are_checked():
                 ([0], [1], [1, 2])):
         with pytest.raises(KernelError):
             copy_moves(*bad, 4, 64)
+
+
+def test_a_job_of_more_blocks_than_a_launch_has_is_refused_before_anything_runs():
+    """On the host: 4 rows' segments of two bytes each in 2^30 entries, or twice as many positions; nothing is read or launched."""
+    from ithaca_b200.csrc import ops
+    lib = ops._search_lib()
+    moves = array.array("i", [0, 1, 1])
+    for job in ([16, 1 << 30, 8, 2, 4, 4, 2, 2, 0, 1], [16, 0x7fffffff, 8, 2, 4, 2, 2, 2, 0, 1]):
+        j = array.array("q", job)
+        assert lib.ik_copy_rows(j.buffer_info()[0], 1, moves.buffer_info()[0], 1, None) == -2
+    j = array.array("q", [16, 1 << 31, 8, 2, 4, 4, 2, 2, 0, 1])
+    assert lib.ik_copy_rows(j.buffer_info()[0], 1, moves.buffer_info()[0], 1, None) == -1
 
 
 # -- who shares pages ------------------------------------------------------------------------------------------------------
@@ -247,6 +275,21 @@ def test_a_captured_step_keeps_room_for_other_groups():
     assert s.starts == [0, 3, 4, 6, 6] and s.n_groups == 4 and s.max_members == 3 and _sharing_shape(s) == (4, 4, 2, 2)
     s = find_sharing(rows([1, 2], [1, 3], [1, 4]), [2, 2, 2])
     assert _sharing_shape(s) == (1, 3, 1, 1)                                       # never more than there are sequences
+
+
+def test_long_runs_are_cut_as_well_as_every_way():
+    """Many neighbours: against the plain search over every last cut."""
+    from ithaca_b200.engine.context import _cut_run
+    rng = random.Random(2)
+    for _ in range(300):
+        c = [rng.randint(1, rng.choice([2, 4, 40])) for _ in range(rng.randint(1, 14)) for _ in range(rng.choice([1, 1, 3]))]
+        best = [0]
+        for j in range(1, len(c) + 2):
+            best.append(max(best[i] + (j - 1 - i) * min(c[i:j - 1], default=0) for i in range(j)))
+        groups = _cut_run(c)
+        assert [a for a, _, _ in groups] == [0] + [b for _, b, _ in groups][:-1] and groups[-1][1] == len(c) + 1
+        assert all(s == min(c[a:b - 1], default=0) for a, b, s in groups) and sum((b - a - 1) * s for a, b, s in groups) == best[-1]
+    assert _cut_run([7] * 500) == [(0, 501, 7)] and _cut_run([]) == [(0, 1, 0)]
 
 
 def test_groups_save_the_most_page_readings():
@@ -390,7 +433,8 @@ def test_stop_tokens_and_budgets():
 
 def test_the_search_refuses():
     be = Backend(8, 1)
-    for bad in (dict(beams=0), dict(beams=17), dict(n_best=0), dict(n_best=5), dict(length_penalty=-1.0), dict(length_penalty=math.nan)):
+    for bad in (dict(beams=0), dict(beams=17), dict(n_best=0), dict(n_best=5), dict(length_penalty=-1.0), dict(length_penalty=math.nan), dict(length_penalty=math.inf),
+                dict(length_penalty=200.0)):
         with pytest.raises(ValueError):
             beam_loop([[1]], BeamOptions(**bad), be)
     for prompts in ([[]], [[1] * 1001]):

@@ -283,3 +283,22 @@ def test_the_command_line_searches(dirs, capsys):
     eng = Engine(dirs("A"), dtype="float32", max_tokens=1024)
     want = eng.beam_search([[1, 2, 3], [9, 8]], beams=3, max_tokens=6, stop_token_ids=[])
     assert capsys.readouterr().out.split() == [",".join(map(str, h[0].tokens)) for h in want]
+
+
+def test_forks_that_share_too_little_step_as_any_others(dirs):
+    """No kernel for shared pages would be chosen, so the captured step is the one that sequences of their own use."""
+    from ithaca_b200 import Engine
+    eng = Engine(dirs("wide"), dtype="bfloat16", max_tokens=64 * 30, max_slots=8)
+    a = eng.alloc_slot()
+    eng.step([a], [random_ids(70, 300, 5)], None)
+    b = eng.fork_slot(a)[0]
+    eng._decoder.step([a, b], [[3], [4]])
+    assert [len(key) for key in eng._decoder.graphs] == [2]
+    eng._settle()
+    ids = random_ids(1, 300, 6)
+    got = eng._decoder.step([a, b], [ids, ids])[0].float().cpu().numpy()
+    alone = [eng.alloc_slot() for _ in range(2)]
+    eng._settle()
+    eng.step(alone, [random_ids(70, 300, 5)] * 2, None)
+    eng.step(alone, [[3], [4]], None)
+    assert off(got, rows(eng, alone, [ids, ids])) <= REL_CUT["bfloat16"]
