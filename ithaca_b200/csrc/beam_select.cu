@@ -7,13 +7,15 @@
 // sums into the beams' lse, and with them every tile's maximum into a score.  Of these the n-th largest is a lower bound of the n-th best candidate (n tiles
 // have a candidate at least as good), and only tiles that are not below it can hold any of the n best: hardly more than n.  Of a tile whose second largest is below the
 // bound the maximum is all that counts; the others are read again (L2 has them) for what is not below it.  What is gathered, usually hardly more than n, is
-// ranked by counting.  A tile gives at most n: one that has more (sorted or constant logits) gives its n best one at a time; where many tiles are as good as the
-// bound, the n best are found by exact comparisons with their places.
+// ranked by counting.  Where there is more (few tiles, sorted or constant logits), a tile's candidates are held against the n-th best of its lanes' two best each, a tile
+// that this does not tell apart gives its n best in sorted lists, and so do all together.  Where many tiles are as good as the bound, the n best are found by exact
+// comparisons with their places.
 //
 // Bound by memory where there are many rows, by the merge's chain of dependent steps where there are few.  us in a replayed graph on B200, tiles + the rest: 32 requests of 16
 // beams over 128,256 tokens 42 + 8 (263 MB: the pass runs at the copy rate), 16 of 8 over 50,257 6.3 + 5.2, one of 4 over 128,256 2.6 + 4.6.  A first version that
 // took every slice's n best by sorting its threads' maxima in the pass itself: 230, 33, 13.  Without a tile's second largest, every chosen tile was read again:
-// 3 to 6 us more.
+// 3 to 6 us more.  Both in one launch, a cluster of 8 or 16 blocks to a request: one of 4 12.6 and 9.8 (7.4 here), 16 of 8 19.  Many candidates a tile: one request of
+// 16 beams over 1,000 tokens, 32 results 11 (85 with the tile's best one at a time and everything ranked by counting); equal logits, 4 beams over 128,256, 32 results 38 (234).
 //
 // Scores are formed and compared in 64 bits (two beams' candidates may be closer than a float of their size can tell) and rounded once;
 // exponentials are floats, summed in float within a tile and in 64 bits beyond.  A logit of -inf or NaN is no candidate; neither is any of a beam
@@ -28,6 +30,7 @@ constexpr int TILE = 1024, PER = TILE / 32;                            // logits
 constexpr int RT = 256, MT = 512, MW = MT / 32;                        // threads of the two kernels
 constexpr int BEAMS = 16, OUT = 32, TILES = 1024;                      // most beams, results and tiles of a row
 constexpr int PICKS = 40;                                              // tiles that the merge takes as they come
+constexpr int CANDS = 160;                                             // candidates that are ranked without a second thought
 
 // What a tile leaves: its maximum, the one behind it (equal to it where it stands twice), the sum of exponentials below the maximum; the maximum's place in its row and the
 // beam in the upper 12 bits.
@@ -132,6 +135,7 @@ __device__ __forceinline__ double order_value(unsigned long long k) {
 }
 __device__ __forceinline__ bool ahead(const Cand& a, const Cand& b) { return (a.s > b.s) | ((a.s == b.s) & (a.at < b.at)); }
 __device__ __forceinline__ Cand shfl_xor(const Cand& c, int m) { return Cand{__shfl_xor_sync(0xffffffffu, c.s, m), __shfl_xor_sync(0xffffffffu, c.at, m)}; }
+__device__ __forceinline__ Cand shfl(const Cand& c, int from) { return Cand{__shfl_sync(0xffffffffu, c.s, from), __shfl_sync(0xffffffffu, c.at, from)}; }
 __device__ __forceinline__ Cand pick(bool second, const Cand& a, const Cand& b) { return Cand{second ? b.s : a.s, second ? b.at : a.at}; }
 __device__ __forceinline__ Cand better(const Cand& a, const Cand& b) { return pick(ahead(b, a), a, b); }
 
@@ -164,6 +168,19 @@ __device__ __forceinline__ T warp_merge(T a, const T& b_reversed, int lane) {
         a = exchange(front, a, o);
     }
     return a;
+}
+
+// The best 32 of the block's warps' sorted lists, in order, at the front of `lists`.
+__device__ __forceinline__ void block_best(Cand list, Cand* lists, int warp, int lane) {
+    lists[warp * 32 + lane] = list;
+    #pragma unroll 1
+    for (int half = MW / 2; half > 0; half >>= 1) {
+        __syncthreads();
+        if (warp < half) list = warp_merge(list, lists[(warp + half) * 32 + 31 - lane], lane);
+        __syncthreads();
+        if (warp < half) lists[warp * 32 + lane] = list;
+    }
+    __syncthreads();
 }
 
 // How many of a list are ahead of its i-th (a warp).
@@ -258,17 +275,8 @@ beam_merge_kernel(const float* __restrict__ logits, long long ldl, const Tile* _
     if (p > PICKS) {                                                   // many equal ones: the bound from the exact order
         Cand mine_best = none();
         for (int i = tid; i < total; i += MT) mine_best = better(mine_best, tile_cand(i));
-        Cand kc = warp_sort(mine_best, lane);
         if (tid == 0) n_picked = 0;
-        cand[warp * 32 + lane] = kc;
-        #pragma unroll 1
-        for (int half = MW / 2; half > 0; half >>= 1) {
-            __syncthreads();
-            if (warp < half) kc = warp_merge(kc, cand[(warp + half) * 32 + 31 - lane], lane);
-            __syncthreads();
-            if (warp < half) cand[warp * 32 + lane] = kc;
-        }
-        __syncthreads();
+        block_best(warp_sort(mine_best, lane), cand, warp, lane);
         const Cand tau = cand[n - 1];
         if (mine_best.s && !ahead(tau, mine_best))
             for (int i = tid; i < total; i += MT) {
@@ -308,40 +316,56 @@ beam_merge_kernel(const float* __restrict__ logits, long long ldl, const Tile* _
         uint32_t in = 0;
         #pragma unroll
         for (int e = 0; e < PER; e++) in |= !(v[e] < least) && v[e] > -INFINITY ? 1u << e : 0u;
-        const int count = __reduce_add_sync(0xffffffffu, __popc(in));
+        int most_of_tile = max(n, CANDS / p), count = __reduce_add_sync(0xffffffffu, __popc(in));
+        if (__builtin_expect(count > most_of_tile, 0)) {                                    // few tiles, or one like no other: the n-th best of the lanes' two best each is a bound, too
+            float top = -INFINITY, next = -INFINITY;
+            #pragma unroll
+            for (int e = 0; e < PER; e++) {
+                const float x = in >> e & 1 ? v[e] : -INFINITY;
+                next = fmaxf(next, fminf(x, top));
+                top = fmaxf(top, x);
+            }
+            const float next_reversed = __shfl_sync(0xffffffffu, warp_sort(next, lane), 31 - lane);
+            const float nth = __shfl_sync(0xffffffffu, warp_merge(warp_sort(top, lane), next_reversed, lane), n - 1);
+            const float tight = (float)((double)nth - 1e-6 * (fabs((double)nth) + fabs(beam.base) + fabs(beam.lse)));      // (as above)
+            #pragma unroll
+            for (int e = 0; e < PER; e++) in &= v[e] < tight ? ~(1u << e) : ~0u;
+            count = __reduce_add_sync(0xffffffffu, __popc(in));
+            most_of_tile = max(n, PICKS * OUT / p);
+        }
         int base = 0;
-        if (lane == 0) base = atomicAdd(&n_cand, min(count, n));
+        if (lane == 0) base = atomicAdd(&n_cand, count <= most_of_tile ? count : n);
         base = __shfl_sync(0xffffffffu, base, 0);
         auto put = [&](int slot, int at) { cand[slot] = cand_of(beam, w[at], (uint32_t)b * (uint32_t)V + (uint32_t)at); };
-        if (count <= n) {
+        if (count <= most_of_tile) {
             int before = __popc(in);
             #pragma unroll
             for (int o = 1; o < 32; o <<= 1) { const int x = __shfl_up_sync(0xffffffffu, before, o); if (lane >= o) before += x; }
             base += before - __popc(in);
             for (; in; in &= in - 1) put(base++, lo + place_in<VEC>(__ffs(in) - 1, lane));
         } else {
-            unsigned long long key[PER];                               // 0: no candidate
-            #pragma unroll
-            for (int e = 0; e < PER; e++) key[e] = in >> e & 1 ? cand_of(beam, v[e], 0).s : 0ull;
+            // the n best in order, 32 logits after the other; by their scores: of large sums several logits give the same
+            Cand list = none();
             #pragma unroll 1
-            for (int j = 0; j < n; j++) {                              // the best that is left.  (By its score: of large sums several logits give the same)
-                Cand top = none();
-                int from = 0;
-                #pragma unroll
-                for (int e = PER - 1; e >= 0; e--)                     // (a lane's places ascend)
-                    if ((in >> e & 1) && key[e] && key[e] >= top.s) { top.s = key[e]; from = e; }
-                if (top.s) top.at = (uint32_t)b * (uint32_t)V + (uint32_t)(lo + place_in<VEC>(from, lane));
-                Cand most = top;
-                #pragma unroll
-                for (int o = 16; o > 0; o >>= 1) most = better(most, shfl_xor(most, o));
-                if (lane == 0) cand[base + j] = most;
-                if (top.at == most.at) in &= ~(1u << from);            // (nothing is left where that is several lanes)
+            for (int e = 0; e < PER; e++) {
+                if (!__any_sync(0xffffffffu, in >> e & 1)) continue;
+                const int at = lo + place_in<VEC>(e, lane);
+                const Cand me = in >> e & 1 ? cand_of(beam, w[at], (uint32_t)b * (uint32_t)V + (uint32_t)at) : none(), last = shfl(list, n - 1);
+                if (!__any_sync(0xffffffffu, ahead(me, last))) continue;
+                list = warp_merge(list, shfl(warp_sort(me, lane), 31 - lane), lane);
             }
+            if (lane < n) cand[base + lane] = list;
         }
     }
     __syncthreads();
     const int c = n_cand;
-    for (int i = warp; i < c; i += MW) {                               // (what turned out to be no candidate stands behind all that are)
+    if (c > CANDS) {                                                   // by counting, 1,024 of them take 150 us
+        Cand list = none();
+        for (int i = warp * 32; i < c; i += MT) list = warp_merge(list, shfl(warp_sort(i + lane < c ? cand[i + lane] : none(), lane), 31 - lane), lane);
+        __syncthreads();
+        block_best(list, cand, warp, lane);
+        if (tid < OUT) order[tid] = tid;
+    } else for (int i = warp; i < c; i += MW) {                        // (what turned out to be no candidate stands behind all that are)
         const int rank = rank_of(cand, c, i, lane);
         if (lane == 0 && rank < n) order[rank] = i;
     }

@@ -108,6 +108,20 @@ def test_select_on_rows_that_are_not_ordinary(kind, R, K, V, n):
     check_select(l, sums, n)
 
 
+@pytest.mark.parametrize("kind", ["random", "few values", "rising", "signed zeros"])
+@pytest.mark.parametrize("R,K,V,n", [(1, 16, 1000, 32), (3, 8, 1001, 16), (2, 16, 1024, 32), (2, 10, 4096, 32), (1, 1, 1000, 32), (5, 2, 33, 32), (2, 16, 2, 32)])
+def test_select_from_few_tiles(kind, R, K, V, n):
+    """Fewer stretches of 1,024 logits than results, or hardly more: many of each one's logits are candidates."""
+    l = torch.randn((R * K, V), generator=gen(V + n)) * 3
+    if kind == "few values":
+        l = (l / 2).round() * 2
+    elif kind == "rising":
+        l = l.sort(1).values
+    elif kind == "signed zeros":
+        l = torch.where(l > 0, 0.0, -0.0)
+    check_select(l, torch.rand((R, K), generator=gen(n)) * -2, n)
+
+
 def test_equal_candidates_come_by_beam_and_token():
     """Equal beams (odd vocabularies: their rows start on different alignments) with equal sums: every rank has an exact tie."""
     for V, n in ((1001, 8), (20003, 32), (128256, 16)):
