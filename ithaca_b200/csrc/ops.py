@@ -1324,40 +1324,42 @@ def copy_rows(jobs) -> None:
     src, dst and positions are host integers.  A row is not written twice, and none is both read and written: such a job is refused, and so are rows out of range
     and jobs whose tensors overlap.  On refusal nothing has been copied."""
     jobs = list(jobs)                              # the lists below are told apart by identity: they have to live until the end
-    table, moves, spans, seen, n_jobs, nbytes = [], [], [], {}, 0, 0
+    table, moves, spans, seen, n_jobs, nbytes, dev = [], [], [], {}, 0, 0, _current_device()
     for t, src, dst, positions in jobs:
-        if not t.is_cuda:
-            raise KernelError("copy_rows: a tensor must be a CUDA tensor (there is no CPU path)")
-        shape, strides, size = t.shape, t.stride(), t.element_size()
+        if t.get_device() != dev:
+            if not t.is_cuda:
+                raise KernelError("copy_rows: a tensor must be a CUDA tensor (there is no CPU path)")
+            _here(t, "copy_rows: a tensor")
+        shape, strides, size, numel = t.shape, t.stride(), t.element_size(), t.numel()
         if len(shape) < 2 or (positions is not None and len(shape) < 4):
             raise KernelError("copy_rows: a tensor is [entries, rows, ...], with positions [entries, rows, heads, page, ...]")
-        _here(t, "copy_rows: a tensor")
-        if len(src) == len(dst) == 0 or t.numel() == 0:
+        if numel == 0 or len(src) == len(dst) == 0:
             continue
-        inner = t.numel() // (shape[0] * shape[1])
+        entries, rows = shape[0], shape[1]
+        inner = numel // (entries * rows)
         if not t.is_contiguous():
             step = 1
             for n, stride in zip(shape[:1:-1], strides[:1:-1]):
                 if n != 1 and stride != step:
                     raise KernelError("copy_rows: behind its first two dimensions a tensor must be contiguous")
                 step *= n
-            if not ((shape[1] == 1 or strides[1] >= inner) and (shape[0] == 1 or strides[0] >= (shape[1] - 1) * strides[1] + inner
-                                                                or (strides[0] >= inner and strides[1] >= (shape[0] - 1) * strides[0] + inner))):
+            if not ((rows == 1 or strides[1] >= inner) and (entries == 1 or strides[0] >= (rows - 1) * strides[1] + inner
+                                                            or (strides[0] >= inner and strides[1] >= (entries - 1) * strides[0] + inner))):
                 raise KernelError("copy_rows: a tensor's rows may not overlap")
         if size % 2:
             raise KernelError("copy_rows: an element must have 2, 4, 8 or 16 bytes")
         heads, page = (1, 1) if positions is None else (shape[2], shape[3])
-        key = (id(src), id(dst), id(positions), shape[1], page)
+        key = (id(src), id(dst), id(positions), rows, page)
         at = seen.get(key)
         if at is None:
             at = seen[key] = len(moves) // 3
-            moves += copy_moves(src, dst, positions, shape[1], page)
-        lo, per_head = t.data_ptr(), inner // heads * size
-        spans.append((lo, lo + ((shape[0] - 1) * strides[0] + (shape[1] - 1) * strides[1] + inner) * size))
-        table += (lo, shape[0], strides[0] * size, shape[1], strides[1] * size, heads, per_head, per_head // page, at, len(src))
+            moves += copy_moves(src, dst, positions, rows, page)
+        lo, per_head, entry, row = t.data_ptr(), inner // heads * size, strides[0] * size, strides[1] * size
+        spans.append((lo, lo + (entries - 1) * entry + (rows - 1) * row + inner * size))
+        table += (lo, entries, entry, rows, row, heads, per_head, per_head // page, at, len(src))
         n_jobs += 1
         if _profile is not None:
-            nbytes += 2 * shape[0] * heads * (per_head // page) * sum(moves[3 * at + 2:3 * (at + len(src)):3])
+            nbytes += 2 * entries * heads * (per_head // page) * sum(moves[3 * at + 2:3 * (at + len(src)):3])
     if not n_jobs:
         return
     if n_jobs > 1:
