@@ -266,7 +266,7 @@ def decode_shared(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                   status: Optional[torch.Tensor], out: Optional[torch.Tensor] = None, softcap: float = 0.0, sink=False,
                   work: Optional[Tuple[int, int]] = None) -> torch.Tensor:
     """Attention of one new token per sequence (``q`` [B, heads * size], bfloat16) over pages of which groups of sequences share the first ones.  ``starts`` int32
-    [n_groups + 1]: group g are the sequences starts[g] <= b < starts[g + 1], at most ``max_members`` of them; ``shared`` int32 [B]: how many of sequence b's first pages are
+    [n_groups + 1]: group g are the sequences starts[g] <= b < starts[g + 1], at most ``max_members`` of them (else ``status`` is set, and those beyond get zeros); ``shared`` int32 [B]: how many of sequence b's first pages are
     the same (and full) in all of its group, 0 for a sequence that shares none; a sequence that is in no group gets zeros.  ``shared_bound``, ``own_bound``: about how many pages a group
     shares and a sequence has of its own at most (for the caller's choice between this and ``decode``, see ``sharing_pays``; the kernel goes by the numbers themselves).  At most 1,024 sequences.  All else
     as ``decode`` has it, without a window."""

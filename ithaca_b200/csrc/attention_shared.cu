@@ -91,7 +91,7 @@ __device__ __forceinline__ float capped(float s, float a, float b) {
 struct Call {
     const int *kv_lens, *table, *starts, *shared;
     int table_stride, table_cols, n_groups, B, nh, nkv, G;
-    int members, heads, head_parts, tiles_per_group, n_tiles;       // members and heads of a tile; parts of the heads; tiles
+    int max_members, members, heads, head_parts, tiles_per_group, n_tiles;       // most members of a group; members and heads of a tile; parts of the heads; tiles
     int runs;
 };
 struct TileOf { int first, last, part, S; };                          // members first <= i < last, part of the heads, pages they share
@@ -191,6 +191,8 @@ attn_shared_kernel(const bf16* __restrict__ q, const bf16* __restrict__ k_pages,
     __syncthreads();
     const Cut cut = cut_of(ends[c.n_tiles - 1], c.runs);
     if (run == 0 && kvh == 0) {
+        for (int i = tid; i < c.n_groups; i += THREADS)
+            if (starts[i] < 0 || starts[i + 1] < starts[i] || starts[i + 1] > c.B || starts[i + 1] - starts[i] > c.max_members) ik_set_status(status, IK_STATUS_BAD_GROUP);
         for (int i = tid; i < c.B; i += THREADS) plan.seqs[i] = make_int2(-1, 0);
         __syncthreads();
         for (int t = tid; t < c.n_tiles; t += THREADS) {
@@ -571,7 +573,7 @@ int launch(const void* q, const void* k_pages, const void* v_pages, void* out, f
 
 // How a call is cut into tiles and runs; RT, or a negative status.
 int cut(Call& c, int n_groups, int max_members, int B, int nh, int nkv) {
-    c.n_groups = n_groups; c.B = B; c.nh = nh; c.nkv = nkv; c.G = nh / nkv;
+    c.n_groups = n_groups; c.max_members = max_members; c.B = B; c.nh = nh; c.nkv = nkv; c.G = nh / nkv;
     const long long rows = (long long)max_members * c.G;
     const int rt = rows <= 16 ? 1 : rows <= 32 ? 2 : 4, most = 16 * rt;
     c.heads = c.G < most ? c.G : most;
@@ -601,7 +603,7 @@ IK_EXPORT long long ik_attn_shared_scratch(int n_groups, int max_members, int B,
     return (long long)(c.n_tiles + c.runs) * nkv * 16 * rt * (HD + 2) * 4 + ((long long)B + c.n_tiles) * 8;
 }
 
-// scratch: ik_attn_shared_scratch bytes on 16 bytes.  starts: [n_groups + 1], shared: [B], on the device; max_members: no group is larger (what is beyond is left out).
+// scratch: ik_attn_shared_scratch bytes on 16 bytes.  starts: [n_groups + 1], shared: [B], on the device; max_members: no group is larger (else *status is set, and what is beyond is left out).
 IK_EXPORT int ik_attn_shared(const void* q, const void* k_pages, const void* v_pages, void* out, void* scratch, const int* kv_lens, const int* table, int table_stride,
                              int table_cols, const int* starts, const int* shared, int n_groups, int max_members, int B, int nh, int nkv, float scale, float softcap,
                              int sink, const float* sink_v, int page_size, int n_pages, int* status, cudaStream_t stream) {

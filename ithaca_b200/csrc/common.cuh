@@ -163,6 +163,7 @@ __device__ __forceinline__ void ik_pdl_wait() { asm volatile("griddepcontrol.wai
 #define IK_STATUS_READ_NO_PAGE 3         // a cache read without a page
 #define IK_STATUS_GEMM_TIMEOUT 4         // a tensor-core block that gave up waiting for its data
 #define IK_STATUS_SMEM_ALIGN 5           // shared memory not aligned for the tensor-core tiles
+#define IK_STATUS_BAD_GROUP 6            // groups of sequences that are larger than the launch was made for, or out of order
 #define IK_STATUS_BIT(code) (1 << ((code) - 1))
 __device__ __forceinline__ void ik_set_status(int* status, int code) { if (status) atomicOr(status, IK_STATUS_BIT(code)); }
 __device__ __forceinline__ bool ik_status_has(const int* status, int code) {

@@ -190,7 +190,8 @@ class Stepper:
 
 STATUS_EVENTS = {1: "a token id outside the vocabulary", 2: "a cache write without a page",
                  3: "a cache read without a page", 4: "a matrix-product block that gave up waiting for its data",
-                 5: "shared memory that is not aligned for the tensor-core tiles"}
+                 5: "shared memory that is not aligned for the tensor-core tiles",
+                 6: "groups of sequences that are larger than was said, or out of order"}
 
 
 def wait_detail(word: int) -> str:

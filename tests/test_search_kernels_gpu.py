@@ -457,6 +457,29 @@ def test_pages_outside_the_pool_are_not_followed():
         assert status.item() == 1 << 2
 
 
+def test_groups_that_are_not_what_was_said_are_reported():
+    """A group of more members than the launch was made for, or bounds out of order: a status, no access elsewhere, and the others as ever."""
+    from ithaca_b200.csrc import attention_bf16
+    from ithaca_b200.engine.step import describe_status
+    g = gen(3)
+    lens = [200] * 6
+    table, total = layout([4, 2], [2, 2], lens, 3)
+    q = torch.randn((6, 4 * 64), generator=g).to(torch.bfloat16).to(DEV)
+    k, v = (torch.randn((total, 2, 64, 64), generator=g).to(torch.bfloat16).to(DEV) for _ in range(2))
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    def run(starts, most):
+        status = torch.zeros(1, dtype=torch.int32, device=DEV)
+        out = attention_bf16.decode_shared(q, k, v, ints(lens), table.to(DEV), ints(starts), ints([2] * 6), len(starts) - 1, most, 2, 2, 4, 64 ** -0.5, status)
+        return out, int(status.item())
+    want, status = run([0, 4, 6], 4)
+    assert status == 0 and run([0, 4, 6, 6], 4)[1] == 0             # an empty group is none
+    for starts, most in (([0, 4, 6], 3), ([0, 4, 7], 4), ([-1, 4, 6], 4), ([0, 4, 2], 4), ([0, 2147483647, 6], 4)):
+        got, status = run(starts, most)
+        assert "groups of sequences" in describe_status(status), (starts, most)
+        assert torch.isfinite(got).all()
+    assert torch.equal(run([0, 4, 6], 3)[0][4:], want[4:])           # (runs of two pages, cut at the same places)
+
+
 def test_shared_attention_replayed_for_other_lengths():
     from ithaca_b200.csrc import attention_bf16
     g = gen(11)
