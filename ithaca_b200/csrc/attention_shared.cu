@@ -46,7 +46,6 @@ constexpr int THREADS = 160;               // four computing warps, one that loa
 constexpr size_t RING = (size_t)NS * STAGE * sizeof(bf16), FIXED = RING + 64 * 8 + 2 * NS * 8 + 8;         // bytes of the ring; with results' maxima and sums, barriers, a flag
 constexpr int JOIN_FAMILY = IK_FAMILY_ELEMENTWISE;
 constexpr int TILES = 1024, SEQS = 1024;   // most tiles and sequences of a launch
-constexpr int LEAST = 2;                   // least pages of a run: a block's set-up and its partial cost about as much as two
 static_assert(HD % 16 == 0 && HD >= 16 && HD <= 256, "head size must be a multiple of 16 up to 256");
 
 __device__ __forceinline__ void cp16(uint32_t smem, const void* gmem, bool valid) {
@@ -123,7 +122,7 @@ __device__ __forceinline__ int pages_in(const int* pages, const TileOf& o) {
 struct Cut { int runs, len, longer; };
 __device__ __forceinline__ Cut cut_of(int pages, int most) {
     Cut c;
-    c.runs = min(most, (pages + LEAST - 1) / LEAST);
+    c.runs = min(most, pages);                                       // (two pages at least to a run: small calls 9.9 us instead of 8.7)
     c.len = pages / max(c.runs, 1);
     c.longer = pages - c.len * c.runs;
     return c;

@@ -477,7 +477,7 @@ def test_groups_that_are_not_what_was_said_are_reported():
         got, status = run(starts, most)
         assert "groups of sequences" in describe_status(status), (starts, most)
         assert torch.isfinite(got).all()
-    assert torch.equal(run([0, 4, 6], 3)[0][4:], want[4:])           # (runs of two pages, cut at the same places)
+    assert torch.equal(run([0, 4, 6], 3)[0][4:], want[4:])           # (a page to a run in both calls)
 
 
 def test_shared_attention_replayed_for_other_lengths():
