@@ -205,7 +205,11 @@ attn_shared_kernel(const bf16* __restrict__ q, const bf16* __restrict__ k_pages,
     if (run >= cut.runs || abort_flag) return;
     const int u_first = run_start(cut, run), u_end = run_start(cut, run + 1);
     int t = 0;
-    while (ends[t] <= u_first) t++;
+    for (int past = c.n_tiles - 1; t < past;) {                       // the first tile that ends behind the run's first page
+        const int mid = (t + past) >> 1;
+        if (ends[mid] <= u_first) t = mid + 1;
+        else past = mid;
+    }
 
     if (warp == 4) {
         // ---- the loader: 32 pages' numbers at a time, one each lane
@@ -485,54 +489,52 @@ attn_shared_kernel(const bf16* __restrict__ q, const bf16* __restrict__ k_pages,
     ik_pdl_launch_dependents();
 }
 
-// Joins a (sequence, head)'s partials, then the sink: a block each, whose groups of HD / 4 threads take every JG-th run and are summed in their order.
+// Joins a (sequence, head)'s partials, then the sink, by groups of HD / 4 threads.  SPLIT: a block each, whose groups take every JG-th run and are summed in their order;
+// else a group each, where the blocks would not fit at a time.  Both, us with the kernel before: 4 sequences of 32 heads in many runs 12.7 / 16.8, 57 31.1 / 31.4, 64 33.4 / 32.7,
+// 256 65 / 60, 1,024 94 / 65.
 constexpr int JV = HD / 4, JG = HD <= 128 ? 128 / JV : 2, JT = JV * JG;
+struct Sum { float4 o; float m, l; };
+__device__ __forceinline__ void add(Sum& s, const float4& v, float m, float l) {
+    const float m_new = fmaxf(s.m, m), m_use = m_new == -INFINITY ? 0.f : m_new, a = ik_ex2(s.m - m_use), w = ik_ex2(m - m_use);
+    s.o = make_float4(s.o.x * a + v.x * w, s.o.y * a + v.y * w, s.o.z * a + v.z * w, s.o.w * a + v.w * w);
+    s.l = s.l * a + l * w;
+    s.m = m_new;
+}
+template <bool SPLIT>
 __global__ void __launch_bounds__(JT)
 attn_shared_join_kernel(const float* __restrict__ part_o, const float2* __restrict__ part_ml, bf16* __restrict__ out, const Plan plan, int rows, int heads, int nh,
                         int nkv, int sink, const float* __restrict__ sink_v) {
-    __shared__ float4 sums[JG][JV];
-    __shared__ float2 ml_of[JG];
+    __shared__ float4 sums[SPLIT ? JG : 1][JV];
+    __shared__ float2 ml_of[SPLIT ? JG : 1];
     ik_pdl_wait();
     ik_pdl_launch_dependents();
     IK_AFTER_WAIT(part_o);
     IK_AFTER_WAIT(part_ml);
-    const int b = blockIdx.x, h = blockIdx.y, G = nh / nkv, grp = threadIdx.x / JV, x = threadIdx.x % JV;
+    const int grp = threadIdx.x / JV, x = threadIdx.x % JV, b = blockIdx.x, h = SPLIT ? blockIdx.y : blockIdx.y * JG + grp, G = nh / nkv;
+    if (!SPLIT && h >= nh) return;
     const int2 where = plan.seqs[b];
     const int in = h % G, t = where.x + in / heads, row = where.y + in % heads, kvh = h / G;
     const int2 over = where.x >= 0 ? plan.tiles[t] : make_int2(1, 0);
-    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    float m = -INFINITY, l = 0.f;
+    const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+    Sum s{zero, -INFINITY, 0.f};
     #pragma unroll 4
-    for (int j = over.x + grp; j <= over.y; j += JG) {
+    for (int j = over.x + (SPLIT ? grp : 0); j <= over.y; j += SPLIT ? JG : 1) {
         const size_t at = ((size_t)(t + j) * nkv + kvh) * rows + row;
         const float2 ml = part_ml[at];
-        float4 v = *reinterpret_cast<const float4*>(part_o + at * HD + x * 4);
-        if (ml.y == 0.f) v = make_float4(0.f, 0.f, 0.f, 0.f);          // a sequence without keys takes nothing from its neighbours' pages, be they infinite
-        const float m_new = fmaxf(m, ml.x), m_use = m_new == -INFINITY ? 0.f : m_new, a = ik_ex2(m - m_use), w = ik_ex2(ml.x - m_use);
-        sum = make_float4(sum.x * a + v.x * w, sum.y * a + v.y * w, sum.z * a + v.z * w, sum.w * a + v.w * w);
-        l = l * a + ml.y * w;
-        m = m_new;
+        const float4 v = *reinterpret_cast<const float4*>(part_o + at * HD + x * 4);
+        add(s, ml.y == 0.f ? zero : v, ml.x, ml.y);                    // a sequence without keys takes nothing from its neighbours' pages, be they infinite
     }
-    sums[grp][x] = sum;
-    if (x == 0) ml_of[grp] = make_float2(m, l);
-    __syncthreads();
-    if (grp != 0) return;
-    const float m_sink = sink ? (sink_v ? sink_v[h] * 1.4426950408889634f : 0.f) : -INFINITY;
-    float mm = m_sink;
-    #pragma unroll
-    for (int i = 0; i < JG; i++) mm = fmaxf(mm, ml_of[i].x);
-    const float m_use = mm == -INFINITY ? 0.f : mm;
-    sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    l = sink ? ik_ex2(m_sink - m_use) : 0.f;
-    #pragma unroll
-    for (int i = 0; i < JG; i++) {
-        const float w = ik_ex2(ml_of[i].x - m_use);
-        const float4 v = sums[i][x];
-        sum.x += v.x * w; sum.y += v.y * w; sum.z += v.z * w; sum.w += v.w * w;
-        l += ml_of[i].y * w;
+    if (SPLIT) {
+        sums[grp][x] = s.o;
+        if (x == 0) ml_of[grp] = make_float2(s.m, s.l);
+        __syncthreads();
+        if (grp != 0) return;
+        #pragma unroll
+        for (int i = 1; i < JG; i++) add(s, sums[i][x], ml_of[i].x, ml_of[i].y);
     }
-    const float inv = l > 0.f ? 1.0f / l : 0.f;                        // (no keys: zeros; a sum that is not a number is passed on below)
-    ik_st4(out, ((size_t)b * nh + h) * HD + x * 4, l == l ? make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv) : make_float4(l, l, l, l));
+    if (sink) add(s, zero, sink_v ? sink_v[h] * 1.4426950408889634f : 0.f, 1.f);
+    const float inv = s.l > 0.f ? 1.0f / s.l : 0.f;                    // (no keys: zeros; a sum that is not a number is passed on below)
+    ik_st4(out, ((size_t)b * nh + h) * HD + x * 4, s.l == s.l ? make_float4(s.o.x * inv, s.o.y * inv, s.o.z * inv, s.o.w * inv) : make_float4(s.l, s.l, s.l, s.l));
 }
 
 template <int RT>
@@ -565,8 +567,9 @@ int launch(const void* q, const void* k_pages, const void* v_pages, void* out, f
     }
     IK_RETURN_IF_ERROR(ik_launch(kern, dim3(c.runs, c.nkv), THREADS, smem, stream, (const bf16*)q, (const bf16*)k_pages, (const bf16*)v_pages, scratch, part_ml, c, plan,
                                  sc_a, sc_b, n_pages, status, map_k, map_v));
-    IK_RETURN_IF_ERROR(ik_launch_family(JOIN_FAMILY, attn_shared_join_kernel, dim3(c.B, c.nh), JT, 0, stream, (const float*)scratch, (const float2*)part_ml, (bf16*)out,
-                                        plan, 16 * RT, c.heads, c.nh, c.nkv, sink, sink_v));
+    const bool split = (long long)c.B * c.nh <= 2048 / JT * ik_sm_count();       // do a block each fit all at a time?
+    IK_RETURN_IF_ERROR(ik_launch_family(JOIN_FAMILY, split ? attn_shared_join_kernel<true> : attn_shared_join_kernel<false>, dim3(c.B, split ? c.nh : (c.nh + JG - 1) / JG), JT, 0,
+                                        stream, (const float*)scratch, (const float2*)part_ml, (bf16*)out, plan, 16 * RT, c.heads, c.nh, c.nkv, sink, sink_v));
     IK_LAUNCH_STATUS();
 }
 

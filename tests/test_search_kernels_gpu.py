@@ -393,6 +393,17 @@ def test_many_groups_of_all_sizes(nh, nkv, hd, seed):
     run_shared(nh, nkv, hd, members, shared, lens, seed=seed)
 
 
+@pytest.mark.parametrize("sink", [False, True])
+@pytest.mark.parametrize("nh,nkv,hd,members", [(64, 8, 16, [3] * 14), (40, 40, 64, [2, 1, 3] * 11), (20, 1, 256, [8] * 17), (6, 3, 80, [5, 1, 2] * 56), (50, 10, 48, [17] * 3), (32, 8, 128, [1] * 80)])
+def test_more_sequences_and_heads_than_blocks_at_a_time(nh, nkv, hd, members, sink):
+    """The join by groups of a block: its last block of heads is not always full."""
+    r = random.Random(nh)
+    shared = [r.randint(0, 3) if m > 1 else 0 for m in members]
+    lens = [64 * s + r.choice([0, 1, 40, 64, 65, 150]) for m, s in zip(members, shared) for _ in range(m)]
+    assert len(lens) * nh > 17 * 148
+    run_shared(nh, nkv, hd, members, shared, lens, seed=nh + hd, sink=torch.randn(nh, generator=gen(nh)) if sink else False)
+
+
 def test_bounds_that_are_too_small_cost_time_only():
     for bounds in ((1, 1), (0, 0), (3, 2), (100, 100)):
         run_shared(8, 2, 64, [3, 2], [7, 4], [449, 500, 700, 257, 300], seed=4, bounds=bounds)
