@@ -489,9 +489,9 @@ attn_shared_kernel(const bf16* __restrict__ q, const bf16* __restrict__ k_pages,
     ik_pdl_launch_dependents();
 }
 
-// Joins a (sequence, head)'s partials, then the sink, by groups of HD / 4 threads.  SPLIT: a block each, whose groups take every JG-th run and are summed in their order;
-// else a group each, where the blocks would not fit at a time.  Both, us with the kernel before: 4 sequences of 32 heads in many runs 12.7 / 16.8, 57 31.1 / 31.4, 64 33.4 / 32.7,
-// 256 65 / 60, 1,024 94 / 65.
+// Joins a (sequence, head)'s partials, then the sink, by groups of HD / 4 threads.  SPLIT: a block each, of so many times JG groups, which share the runs out and are summed in
+// their order; 0: a group each.  us with the kernel before, twice JG / JG / a group: 4 sequences of 32 heads 11.3 / 12.4 / 16.8, 18 15.1 / 15.3 / 17.5, 32 39.7 / 38.5 / 38.6, 64 35.3 /
+// 33.7 / 32.7, 256 72 / 66 / 60, 1,024 120 / 94 / 65.
 constexpr int JV = HD / 4, JG = HD <= 128 ? 128 / JV : 2, JT = JV * JG;
 struct Sum { float4 o; float m, l; };
 __device__ __forceinline__ void add(Sum& s, const float4& v, float m, float l) {
@@ -500,12 +500,13 @@ __device__ __forceinline__ void add(Sum& s, const float4& v, float m, float l) {
     s.l = s.l * a + l * w;
     s.m = m_new;
 }
-template <bool SPLIT>
-__global__ void __launch_bounds__(JT)
+template <int SPLIT>
+__global__ void __launch_bounds__(JT * (SPLIT ? SPLIT : 1))
 attn_shared_join_kernel(const float* __restrict__ part_o, const float2* __restrict__ part_ml, bf16* __restrict__ out, const Plan plan, int rows, int heads, int nh,
                         int nkv, int sink, const float* __restrict__ sink_v) {
-    __shared__ float4 sums[SPLIT ? JG : 1][JV];
-    __shared__ float2 ml_of[SPLIT ? JG : 1];
+    constexpr int GROUPS = SPLIT ? JG * SPLIT : 1;                     // of a head
+    __shared__ float4 sums[GROUPS][JV];
+    __shared__ float2 ml_of[GROUPS];
     ik_pdl_wait();
     ik_pdl_launch_dependents();
     IK_AFTER_WAIT(part_o);
@@ -518,7 +519,7 @@ attn_shared_join_kernel(const float* __restrict__ part_o, const float2* __restri
     const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
     Sum s{zero, -INFINITY, 0.f};
     #pragma unroll 4
-    for (int j = over.x + (SPLIT ? grp : 0); j <= over.y; j += SPLIT ? JG : 1) {
+    for (int j = over.x + (SPLIT ? grp : 0); j <= over.y; j += GROUPS) {
         const size_t at = ((size_t)(t + j) * nkv + kvh) * rows + row;
         const float2 ml = part_ml[at];
         const float4 v = *reinterpret_cast<const float4*>(part_o + at * HD + x * 4);
@@ -530,7 +531,7 @@ attn_shared_join_kernel(const float* __restrict__ part_o, const float2* __restri
         __syncthreads();
         if (grp != 0) return;
         #pragma unroll
-        for (int i = 1; i < JG; i++) add(s, sums[i][x], ml_of[i].x, ml_of[i].y);
+        for (int i = 1; i < GROUPS; i++) add(s, sums[i][x], ml_of[i].x, ml_of[i].y);
     }
     if (sink) add(s, zero, sink_v ? sink_v[h] * 1.4426950408889634f : 0.f, 1.f);
     const float inv = s.l > 0.f ? 1.0f / s.l : 0.f;                    // (no keys: zeros; a sum that is not a number is passed on below)
@@ -567,8 +568,11 @@ int launch(const void* q, const void* k_pages, const void* v_pages, void* out, f
     }
     IK_RETURN_IF_ERROR(ik_launch(kern, dim3(c.runs, c.nkv), THREADS, smem, stream, (const bf16*)q, (const bf16*)k_pages, (const bf16*)v_pages, scratch, part_ml, c, plan,
                                  sc_a, sc_b, n_pages, status, map_k, map_v));
-    const bool split = (long long)c.B * c.nh <= 2048 / JT * ik_sm_count();       // do a block each fit all at a time?
-    IK_RETURN_IF_ERROR(ik_launch_family(JOIN_FAMILY, split ? attn_shared_join_kernel<true> : attn_shared_join_kernel<false>, dim3(c.B, split ? c.nh : (c.nh + JG - 1) / JG), JT, 0,
+    // a group each where blocks of a head each would not fit at a time; of twice the threads where they take a quarter of the space
+    const long long place = 2048ll / JT * ik_sm_count(), blocks = (long long)c.B * c.nh;
+    const int split = blocks * 4 <= place ? 2 : blocks <= place ? 1 : 0;
+    auto join = split == 2 ? attn_shared_join_kernel<2> : split == 1 ? attn_shared_join_kernel<1> : attn_shared_join_kernel<0>;
+    IK_RETURN_IF_ERROR(ik_launch_family(JOIN_FAMILY, join, dim3(c.B, split ? c.nh : (c.nh + JG - 1) / JG), JT * (split ? split : 1), 0,
                                         stream, (const float*)scratch, (const float2*)part_ml, (bf16*)out, plan, 16 * RT, c.heads, c.nh, c.nkv, sink, sink_v));
     IK_LAUNCH_STATUS();
 }
