@@ -245,18 +245,18 @@ SHARED_SEQS_MOST = SHARED_TILES_MOST = 1024          # what one launch of the ke
 def sharing_pays(n_seqs: int, n_groups: int, max_members: int, shared_bound: int, own_bound: int, n_heads: int, n_kv_heads: int, hd: int) -> bool:
     """Whether a decode step whose sequences share pages reads them once per group (``decode_shared``), from the sizes that a captured step is kept under.
 
-    It saves (n_seqs - n_groups) readings of the shared pages per kv head, and costs 2 to 4 us more to set up; pages of one's own cost more there the more rows a tile
-    has (all warps pass them, few have work).  us on B200, ``decode`` / ``decode_shared``, pages shared + own: 32 heads of 128 on 8, one group of 4: 8+1 9.3 / 9.4,
-    16+1 11.3 / 10.3, 48+1 16.7 / 12.4; four of 2: 4+1 9.5 / 8.8, 8+1 11.2 / 10.2; four of 8: 2+1 10.9 / 11.6, 4+1 13.9 / 11.8, 2+4 15.4 / 18.3, 4+4 18.2 / 15.9; four of 16:
-    2+1 19.1 / 15.2, 4+4 29.6 / 33.1, 8+4 38.9 / 27.5; sixteen of 4: 1+4 23.7 / 20.9, 48+4 127 / 54; 40 heads on 40, four of 16: 48+1 530 / 61.  32 heads of 64: one
-    group of 4: 16+1 9.3 / 8.9; four of 4: 4+1 8.6 / 8.3, 8+1 10.1 / 8.9.  Over 396 such combinations the choice is 0.7 % behind the better one on average, 24 % at worst."""
+    It saves (n_seqs - n_groups) readings of the shared pages per kv head, and costs 1 to 3 us more to set up; with more than 32 rows to a tile pages of one's own cost
+    more there, too (all warps pass them, few have work).  us on B200, ``decode`` / ``decode_shared``, pages shared + own: 32 heads of 128 on 8, one group of 4: 8+1 9.1 / 9.3,
+    16+1 11.2 / 9.9, 48+1 16.5 / 11.3; four of 2: 4+1 9.5 / 8.6, 8+1 11.3 / 9.6; four of 8: 2+1 10.9 / 11.7, 4+1 13.8 / 12.0, 2+4 15.4 / 18.7, 4+4 18.2 / 16.1; four of 16:
+    2+1 18.6 / 15.7, 4+4 29.5 / 33.2, 8+4 38.9 / 27.9; sixteen of 4: 1+4 23.7 / 21.3, 48+4 127 / 55; 40 heads on 40, four of 16: 48+1 529 / 61.  32 heads of 64: one
+    group of 4: 16+1 9.1 / 8.8; four of 4: 4+1 8.6 / 8.8, 8+1 10.1 / 9.2.  Over 396 such combinations the choice is 0.5 % behind the better one on average, 23 % at worst."""
     rows = max_members * (n_heads // n_kv_heads)
     tall = 16 if rows <= 16 else 32 if rows <= 32 else 64
     heads = min(n_heads // n_kv_heads, tall)
     tiles = n_groups * -(-max_members // max(1, min(tall // heads, max_members))) * -(-(n_heads // n_kv_heads) // heads)
     if n_seqs > SHARED_SEQS_MOST or tiles > SHARED_TILES_MOST:
         return False
-    least, each = {16: (224, 0.05), 32: (384, 0.4), 64: (512, 0.75)}[tall]
+    least, each = {16: (224, 0.0), 32: (512, 0.0), 64: (512, 0.75)}[tall]
     saved, own = (n_seqs - n_groups) * shared_bound * n_kv_heads, n_seqs * own_bound * n_kv_heads
     return saved * (hd + 64) / 192 >= least + each * own
 
