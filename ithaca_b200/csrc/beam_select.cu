@@ -275,6 +275,7 @@ beam_merge_kernel(const float* __restrict__ logits, long long ldl, const Tile* _
     if (p > PICKS) {                                                   // many equal ones: the bound from the exact order
         Cand mine_best = none();
         for (int i = tid; i < total; i += MT) mine_best = better(mine_best, tile_cand(i));
+        __syncthreads();                                               // every thread has read the number that is counted anew
         if (tid == 0) n_picked = 0;
         block_best(warp_sort(mine_best, lane), cand, warp, lane);
         const Cand tau = cand[n - 1];
