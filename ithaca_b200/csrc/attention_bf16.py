@@ -276,8 +276,10 @@ def decode_shared(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
         raise KernelError("decode_shared: pages of 64 keys and values of one head size, a multiple of 16 up to 256, are supported")
     if n_heads % nkv or q.numel() != B * n_heads * hd:
         raise KernelError(f"decode_shared: queries {tuple(q.shape)} are not {B} times {n_heads} heads of {hd} on {nkv} kv heads")
-    dev = ops._current_device()
-    for t, name, dtype in ((q, "q", bf16), (k_pages, "k_pages", bf16), (v_pages, "v_pages", bf16), (kv_lens, "kv_lens", i32), (starts, "starts", i32), (shared, "shared", i32)):
+    ops._need(q, "q", bf16)
+    ops._here(q, "q")
+    dev = q.get_device()
+    for t, name, dtype in ((k_pages, "k_pages", bf16), (v_pages, "v_pages", bf16), (kv_lens, "kv_lens", i32), (starts, "starts", i32), (shared, "shared", i32)):
         if t.dtype is not dtype or t.get_device() != dev or not t.is_contiguous():       # (-1 on the host)
             ops._need(t, name, dtype)
             ops._here(t, name)

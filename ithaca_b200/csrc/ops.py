@@ -35,12 +35,13 @@ def _ptr(t: Optional[torch.Tensor]) -> int:
     return 0 if t is None else t.data_ptr()
 
 
-_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+def _current_device() -> int:
+    return torch._C._cuda_getDevice()              # (looked up here: a torch built without CUDA has neither of the two names, and this module is imported there, too)
 
 
 def _stream() -> int:
     """The current stream of the current device.  (Asked for without a ``torch.cuda.Stream`` object around it, which costs 3 us a call.)"""
-    return _raw_stream(_current_device())
+    return torch._C._cuda_getCurrentRawStream(_current_device())
 
 
 def _need(t: torch.Tensor, name: str, dtype=None, contiguous: bool = True) -> None:
@@ -1262,8 +1263,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n_out: int, out: Opt
     of its softmax probability.  Returns (scores [R, n_out] float32, beams [R, n_out] int32, tokens [R, n_out] int32) of the
     best, descending, equal ones by ascending (beam, token); places without a candidate hold -inf, -1, -1.  Tokens whose logit is -inf or NaN are
     no candidates, nor is what scores below a float32's range.  ``out``: int32 [3, R, n_out] to write into (the scores' bits first); the results are views of it."""
-    dev = _current_device()
-    if not (logits.dtype is scores.dtype is torch.float32 and logits.get_device() == scores.get_device() == dev and scores.is_contiguous()):       # (-1 on the host)
+    dev = logits.get_device()                      # -1 on the host
+    if not (logits.dtype is scores.dtype is torch.float32 and dev == scores.get_device() and dev >= 0 and dev == _current_device() and scores.is_contiguous()):
         _need(logits, "logits", torch.float32, contiguous=False)
         _need(scores, "scores", torch.float32)
         _here(logits, "logits")
@@ -1324,12 +1325,13 @@ def copy_rows(jobs) -> None:
     src, dst and positions are host integers.  A row is not written twice, and none is both read and written: such a job is refused, and so are rows out of range
     and jobs whose tensors overlap.  On refusal nothing has been copied."""
     jobs = list(jobs)                              # the lists below are told apart by identity: they have to live until the end
-    table, moves, spans, seen, n_jobs, nbytes, dev = [], [], [], {}, 0, 0, _current_device()
+    table, moves, spans, seen, n_jobs, nbytes, dev = [], [], [], {}, 0, 0, -1
     for t, src, dst, positions in jobs:
-        if t.get_device() != dev:
+        if t.get_device() != dev or dev < 0:
             if not t.is_cuda:
                 raise KernelError("copy_rows: a tensor must be a CUDA tensor (there is no CPU path)")
             _here(t, "copy_rows: a tensor")
+            dev = t.get_device()
         shape, strides, size, numel = t.shape, t.stride(), t.element_size(), t.numel()
         if len(shape) < 2 or (positions is not None and len(shape) < 4):
             raise KernelError("copy_rows: a tensor is [entries, rows, ...], with positions [entries, rows, heads, page, ...]")
