@@ -22,7 +22,8 @@ BEAMS_MOST, CHOICES_MOST = 16, 32          # what the kernel that chooses takes
 class BeamOptions:
     """``beams``: beams per request.  A hypothesis is ranked by its log probability divided by its length (new tokens, the stop token included) to the
     power ``length_penalty``.  A request ends when it has ``beams`` hypotheses and no beam can still rank above the worst of
-    them by what it has now (``early_stopping``: as soon as it has them), or at ``max_tokens``, where its beams become hypotheses as they stand."""
+    them by what it has now (``early_stopping``: as soon as it has them), or at ``max_tokens``, where its beams become hypotheses as they stand.  Beams and
+    stop tokens together may be 32 at most."""
     beams: int = 4
     max_tokens: int = 128
     length_penalty: float = 1.0
@@ -90,6 +91,11 @@ def ranked(logprob: float, length: int, penalty: float) -> float:
     return logprob / max(1, length) ** penalty
 
 
+def joined(choices: Sequence[Sequence[Tuple[float, int, int]]]) -> List[Tuple[float, int, int]]:
+    """The choices of beams that were asked one by one, as those of one request: best first, equal ones by beam, of a beam in their order."""
+    return sorted(((score, beam, token) for beam, found in enumerate(choices) for score, _, token in found), key=lambda c: -c[0])
+
+
 def beam_loop(prompts: Sequence[Sequence[int]], options: BeamOptions, backend: BeamBackend, stop_token_ids: Sequence[int] = (),
               clock: Callable[[], float] = time.perf_counter):
     """Returns (hypotheses per request, best first, at most ``n_best``; GenStats)."""
@@ -102,8 +108,14 @@ def beam_loop(prompts: Sequence[Sequence[int]], options: BeamOptions, backend: B
         if len(p) > ctx:
             raise ValueError(f"request {n}: the prompt of {len(p)} tokens is longer than the context of {ctx}")
     budgets = [budget_for(len(p), o.max_tokens, ctx) for p in prompts]
-    # of so many choices at least K are no stop tokens (as far as the kernel goes)
-    n_out = min(CHOICES_MOST, o.beams * (1 + len(stops)))
+    # of so many choices at least K are no stop tokens.  Where the kernel does not give so many, every beam is asked for its own: K of them are no stop tokens, and the best
+    # of all beams are among them
+    n_out = o.beams * (1 + len(stops))
+    apart = n_out > CHOICES_MOST
+    if apart:
+        n_out = o.beams + len(stops)
+        if n_out > CHOICES_MOST:
+            raise ValueError(f"{o.beams} beams and {len(stops)} stop tokens: at most {CHOICES_MOST} together are supported")
     results: List[List[Hypothesis]] = [[] for _ in prompts]
     stats = GenStats()
     pending = list(range(len(prompts)))
@@ -183,7 +195,11 @@ def beam_loop(prompts: Sequence[Sequence[int]], options: BeamOptions, backend: B
                 running.sort(key=lambda run: len(run.beams))               # as many beams next to one another; else in their order
                 beams = [b for run in running for b in run.beams]
                 tokens = [list(prompts[run.request]) for run in running] if first else [[b.tokens[-1]] for b in beams]
-                picked = backend.step_and_select([b.slot for b in beams], tokens, [[b.score for b in run.beams] for run in running], n_out)
+                if apart:
+                    each = iter(backend.step_and_select([b.slot for b in beams], tokens, [[b.score] for b in beams], n_out))
+                    picked = [joined([next(each) for _ in run.beams]) for run in running]
+                else:
+                    picked = backend.step_and_select([b.slot for b in beams], tokens, [[b.score for b in run.beams] for run in running], n_out)
                 running = advance(running, [settle(run, c) for run, c in zip(running, picked)])
                 stats.steps += 1
                 if first:
