@@ -96,7 +96,7 @@ struct Call {
 struct TileOf { int first, last, part, S; };                          // members first <= i < last, part of the heads, pages they share
 __device__ __forceinline__ TileOf tile_of(const Call& c, const int* starts, const int* shared, int t) {
     const int g = t / c.tiles_per_group, k = t % c.tiles_per_group;
-    const int a = min(max(starts[g], 0), c.B), b = min(max(starts[g + 1], a), c.B);
+    const int a = min(max(starts[g], 0), c.B), b = min(max(starts[g + 1], a), min(c.B, a + c.max_members));       // (a part of its last tile may lie beyond the bound)
     TileOf o;
     o.part = k % c.head_parts;
     o.first = min(a + k / c.head_parts * c.members, b);
