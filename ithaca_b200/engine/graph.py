@@ -90,6 +90,12 @@ def _sharing_shape(f: Optional[Sharing]):
     return min(B, _above(f.n_groups)), min(B, _above(f.max_members)), _above(f.shared_bound), _above(f.own_bound)
 
 
+def _round_up(f: Sharing) -> None:
+    """Makes of who shares pages what a captured step takes: as for the lengths, the kernels and the sizes of grids follow from the shape the graph is kept under."""
+    groups, f.most, f.shared_bound, f.own_bound = _sharing_shape(f)
+    f.pad(groups)
+
+
 class GraphDecoder:
     def __init__(self, stepper: Stepper):
         self.stepper = stepper
@@ -202,10 +208,7 @@ class GraphDecoder:
             cols = _bucket(int(-(-(int(lens.max()) + 1) // page)))
             sharing = []
             if any(pool.n_shared for pool in table.pools):
-                sharing = st.sharing([t[idx, :cols] for t in table.tables], (lens // page + 1).tolist())
-                for f in sharing:
-                    if f is not None:
-                        f.pad(_sharing_shape(f)[0])
+                sharing = st.sharing([t[idx, :cols] for t in table.tables], (lens // page + 1).tolist(), _round_up)
             key = (B, cols) + tuple(_sharing_shape(f) for f in sharing)
             cap = self.graphs.get(key)
             if cap is None:
@@ -281,12 +284,10 @@ class GraphDecoder:
         # room for who shares pages: up to B groups in every key/value group (the buffer may be longer than what it describes)
         room = field_offsets([B, B, B, B + 1, B, B, B] + [B * cols] * n_groups + [B + 1, B] * n_groups)[2]
         buffer = torch.empty(room, dtype=torch.int32, device=st.runtime.device)
-        ctx = st.prepare(slots, tokens, "last", into=buffer, table_cols=cols, pad=lambda f: f.pad(_sharing_shape(f)[0]))
+        ctx = st.prepare(slots, tokens, "last", into=buffer, table_cols=cols, round_up=_round_up)
         sharing = [f for f in ctx.sharing if f is not None]
         offsets, sizes, total = field_offsets([B, B, B, B + 1, B, B, B] + [B * cols] * n_groups + [n for f in sharing for n in (len(f.starts), B)])
         buffer = buffer[:total]
-        for f in sharing:                                     # as for the lengths: sizes of grids follow from the shape the graph is kept under
-            _, f.most, f.shared_bound, f.own_bound = _sharing_shape(f)
         # the graph is replayed for other lengths: what the kernels choose for it follows from its shape alone, not from which lengths came first
         ctx.kv_len_bound, ctx.replayed = cols * page, True
         torch.cuda.current_stream().synchronize()

@@ -9,7 +9,7 @@ does for the last row (src/model.cpp:1588-1594).
 from __future__ import annotations
 
 import dataclasses
-from typing import Dict, List, Mapping, Optional
+from typing import Dict, List, Mapping, Optional, Set
 
 import torch
 
@@ -104,6 +104,15 @@ class DecoderModel:
                         have = out[e.cache][n] = dataclasses.replace(have, window=r.window)
                     if isinstance(have, KVRequest) and r.keep_first > have.keep_first:
                         out[e.cache][n] = dataclasses.replace(have, keep_first=r.keep_first)
+        return out
+
+    def joint_heads(self) -> Dict[int, Set[int]]:
+        """Per cache entry the numbers of query heads of the runs that may read pages which sequences share once."""
+        out: Dict[int, Set[int]] = {}
+        for e in self.spec.schedule:
+            heads = getattr(self.layers[e.layer].mixer, "joint_heads", 0)
+            if heads:
+                out.setdefault(e.cache, set()).add(heads)
         return out
 
     def forward(self, ctx, cache: SequenceCache) -> Optional[torch.Tensor]:

@@ -12,7 +12,7 @@ tokens the step brings, so what else is in the batch cannot change a row.
 """
 from __future__ import annotations
 
-from typing import List, Optional, Sequence, Union
+from typing import Callable, List, Optional, Sequence, Union
 
 import numpy as np
 import torch
@@ -43,6 +43,9 @@ class Stepper:
         self.vocab_size = model.spec.vocab_size
         self.max_position = max_position if max_position is not None else model.spec.max_position
         self.builder = ContextBuilder(self.runtime.device)
+        joint = model.joint_heads() if hasattr(model, "joint_heads") else {}
+        # per key/value group: query heads of the layers whose kernels may read shared pages once
+        self.joint_heads = [set().union(*(joint.get(e, ()) for e in g.cache_entries)) for g in cache.kv_groups]
 
     # -- validation (host only; nothing has changed when it raises) ----------------------------
     def _validate(self, slots, tokens, want) -> List[List[int]]:
@@ -79,8 +82,8 @@ class Stepper:
 
     def prepare(self, slots: Sequence[int], tokens: Sequence[Sequence[int]],
                 want: Union[str, None, Sequence[Sequence[int]]] = "last",
-                into: Optional[torch.Tensor] = None, table_cols: Optional[int] = None, pad=None) -> StepContext:
-        """Validates, reserves pages and uploads the step's description.  ``pad``: is handed who shares pages before that is uploaded (a captured step keeps room)."""
+                into: Optional[torch.Tensor] = None, table_cols: Optional[int] = None, round_up: Optional[Callable[[Sharing], None]] = None) -> StepContext:
+        """Validates, reserves pages and uploads the step's description.  ``round_up``: see ``sharing``."""
         want_lists = self._validate(slots, tokens, want)
         n_new = [len(t) for t in tokens]
         self.cache.reserve(slots, n_new)
@@ -92,27 +95,26 @@ class Stepper:
                 raise StepError("the block table is narrower than the longest sequence")
             cols = table_cols
         tables = [self.cache.table.table_rows(g, slots, cols) for g in range(len(self.cache.kv_groups))]
-        sharing = self.sharing(tables, [-(-(st + 1) // page) for st in start]) if all(n == 1 for n in n_new) else ()
-        for f in sharing:
-            if pad is not None and f is not None:
-                pad(f)
+        sharing = self.sharing(tables, [-(-(st + 1) // page) for st in start], round_up) if all(n == 1 for n in n_new) else ()
         return self.builder.build(slots, tokens, start, want_lists, tables, into=into, sharing=sharing)
 
-    def sharing(self, tables: Sequence[np.ndarray], n_pages: Sequence[int]) -> List[Optional[Sharing]]:
-        """Per key/value group which neighbours of a decode step share pages, where a kernel reads such pages once; an empty list if there are none.  ``tables``:
-        the step's block tables, ``n_pages``: the pages of each sequence."""
+    def sharing(self, tables: Sequence[np.ndarray], n_pages: Sequence[int], round_up: Optional[Callable[[Sharing], None]] = None) -> List[Optional[Sharing]]:
+        """Per key/value group which neighbours of a decode step share pages, where a layer's kernel will read such pages once; an empty list if there are none: the
+        step is as any other then.  ``tables``: the step's block tables, ``n_pages``: the pages of each sequence, ``round_up``: makes of the sizes those that a captured step is kept
+        under (the kernel is chosen by them)."""
         out: List[Optional[Sharing]] = []
         if self.runtime.dtype != "bfloat16" or not any(pool.n_shared for pool in self.cache.table.pools):
             return out
         from ..csrc import attention_bf16
-        for grp, pool, t in zip(self.cache.kv_groups, self.cache.table.pools, tables):
+        for grp, pool, t, joint in zip(self.cache.kv_groups, self.cache.table.pools, tables, self.joint_heads):
             found = None
-            if (pool.n_shared and grp.window is None and not grp.key_scales and grp.v_head_dim in (None, grp.head_dim) and self.cache.page_size == 64
+            if (joint and pool.n_shared and grp.window is None and not grp.key_scales and grp.v_head_dim in (None, grp.head_dim) and self.cache.page_size == 64
                     and attention_bf16.supported(grp.head_dim)):
                 found = find_sharing(t, n_pages)
-                # too little for any number of heads, and a captured step rounds the shared pages up to less than twice as many: the step is as any other
-                if found is not None and not attention_bf16.sharing_pays(len(n_pages), found.n_groups, found.max_members, 2 * found.shared_bound, 0,
-                                                                         grp.n_kv_heads, grp.n_kv_heads, grp.head_dim):
+                if found is not None and round_up is not None:
+                    round_up(found)
+                if found is not None and not any(attention_bf16.sharing_pays(len(n_pages), found.n_groups, found.max_members, found.shared_bound, found.own_bound, heads,
+                                                                             grp.n_kv_heads, grp.head_dim) for heads in joint):
                     found = None
             out.append(found)
         return out if any(f is not None for f in out) else []

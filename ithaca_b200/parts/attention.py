@@ -245,6 +245,11 @@ class Attention:
         att = self._attend_wide(p, ctx, cache, writes_cache)
         ops.head_gate(att, p if self.head_gate else None, self.g_off, mid, self.n_heads, mult, wide=self.gate_wide)
 
+    @property
+    def joint_heads(self) -> int:
+        """Query heads whose decode steps may read pages that sequences share once (0: this layer's kernels read them per sequence)."""
+        return 0 if self.window or self.slopes is not None or self.values_are_keys or self.v_head_dim != self.head_dim else self.n_heads
+
     def cache_requests(self) -> List[object]:
         v = self.v_head_dim if self.v_head_dim != self.head_dim else None
         out: List[object] = [KVRequest(self.n_kv_heads, self.head_dim, self.window, v, values_in_keys=self.values_are_keys,

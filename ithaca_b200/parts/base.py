@@ -17,7 +17,8 @@ method that states the tensors it needs with their shapes, and a constructor
 * mixer:         ``cache_requests() -> [KVRequest | StateRequest, ...]`` and
                  ``forward(x, ctx, cache, residual, writes_cache)``: reads the normed
                  activations ``x[T, d]``, updates its cache entry for the step's tokens,
-                 and adds its output into ``residual[T, d]`` (float32).
+                 and adds its output into ``residual[T, d]`` (float32).  One that calls ``attention.attend`` may
+                 have ``joint_heads``: its query heads, if forked sequences' shared pages may be read once.
 * feed-forward:  ``forward(x, ctx, residual)``: adds its output into ``residual``.
 * block:         ``forward(residual, ctx, cache, writes_cache)``: arranges norms, mixer and
                  feed-forward around the residual stream.

@@ -95,6 +95,10 @@ class ParallelMixer:
     def graph_safe(self) -> bool:
         return all(getattr(br, "graph_safe", False) for br in self.branches)
 
+    @property
+    def joint_heads(self) -> int:
+        return max(getattr(br, "joint_heads", 0) for br in self.branches)              # (one branch at most keeps keys and values)
+
     def cache_requests(self) -> List[object]:
         return [r for br in self.branches for r in br.cache_requests()]
 
