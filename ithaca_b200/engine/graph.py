@@ -96,6 +96,9 @@ def _round_up(f: Sharing) -> None:
     f.pad(groups)
 
 
+SHARED_KEPT = 64          # captured steps of sequences that share pages; a search over many requests meets 4 to 6 a width and number of sequences
+
+
 class GraphDecoder:
     def __init__(self, stepper: Stepper):
         self.stepper = stepper
@@ -215,9 +218,11 @@ class GraphDecoder:
                 if tokens is None:
                     return None                               # a new shape is captured with real tokens only
                 cap = self._capture(slots, [[t] for t in tokens], cols)
-                self.graphs[key] = cap
+                self._keep(key, cap)
                 self.launches_last_step = cap.launches
                 return cap
+            if sharing:
+                self.graphs[key] = self.graphs.pop(key)       # the last one used
             # pages: a sequence needs a new one only when it stands at a page boundary
             for s in idx[table._reserved[idx] <= lens]:
                 table.reserve(int(s), 1)
@@ -272,6 +277,15 @@ class GraphDecoder:
             table.length[idx] += 1
         self.launches_last_step = cap.launches
         return cap
+
+    def _keep(self, key: tuple, cap: _Captured) -> None:
+        """Keeps a step that was just captured (nothing is in flight).  Of those of sequences that share pages the one that was not used for longest goes when there are
+        ``SHARED_KEPT``: the ways of sharing have no end, while numbers of sequences and widths have one."""
+        if len(key) > 2:
+            kept = [k for k in self.graphs if len(k) > 2]
+            for old in kept[:max(0, len(kept) + 1 - SHARED_KEPT)]:
+                del self.graphs[old]
+        self.graphs[key] = cap
 
     def _capture(self, slots, tokens, cols) -> _Captured:
         """The first step of a shape runs eagerly (it also compiles whatever the model still
