@@ -247,14 +247,16 @@ class Engine:
 
     def step_and_select(self, slots, tokens, scores, n_out):
         """One step and the choice behind it.  ``slots``, ``tokens``: all beams' of all requests, a request's next to one another; ``scores``: per request its beams' sums.  Returns per
-        request a list of (score, beam, token), best first."""
+        request a list of (score, beam, token), best first.  The kernel takes and gives floats: a request's sums are handed to it as differences from the best of them, so that what a
+        long search has added up does not cost the next token's probability its last bits."""
         if self._decoder is not None and all(len(t) == 1 for t in tokens):
             logits, _ = self._decoder.step(slots, tokens)
         else:
             self._settle()
             logits = self.stepper.step(slots, tokens, "last")
         outs, row = [], 0
-        sums = torch.tensor([x for s in scores for x in s], dtype=torch.float32).pin_memory().to(logits.device, non_blocking=True)
+        best = [max(s) for s in scores]
+        sums = torch.tensor([x - b for s, b in zip(scores, best) for x in s], dtype=torch.float32).pin_memory().to(logits.device, non_blocking=True)
         at = 0
         while at < len(scores):                                 # neighbours with as many beams are one call
             K, end = len(scores[at]), at
@@ -269,7 +271,7 @@ class Engine:
         for out in outs:
             host = out.cpu()                                    # waits for the step
             for s, b, v in zip(host[0].view(torch.float32).tolist(), host[1].tolist(), host[2].tolist()):
-                picked.append([x for x in zip(s, b, v) if x[1] >= 0])
+                picked.append([(best[len(picked)] + x, beam, token) for x, beam, token in zip(s, b, v) if beam >= 0])
         self.stepper.check_status()
         return picked
 
