@@ -285,6 +285,10 @@ def decode_shared(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
             ops._here(t, name)
     ops._need(table, "table", i32, contiguous=False)
     ops._here(table, "table")
+    for t, name, dtype in ((status, "status", i32), (ops.sink_values(sink, n_heads), "the sink", torch.float32)):
+        if t is not None:                          # (handed to the kernel as an address, like the rest)
+            ops._need(t, name, dtype)
+            ops._here(t, name)
     if starts.numel() != n_groups + 1 or shared.numel() != B:
         raise KernelError(f"decode_shared: {n_groups + 1} starts and {B} numbers of shared pages are needed, found {starts.numel()} and {shared.numel()}")
     if shared_bound < 0 or own_bound < 0:
