@@ -197,7 +197,7 @@ class SequenceCache:
         if self.state_groups and n not in (0, self.length(slot)):
             raise CacheError("a sequence with fixed-size state can only be truncated to 0")
         shorter = n < self.length(slot)
-        self._copy(self.table.truncate(slot, n), [], [])
+        self.table.truncate(slot, n, lambda pages: self._copy(pages, [], []))
         if n == 0 and shorter:
             for t in self.state:
                 t[:, slot].zero_()

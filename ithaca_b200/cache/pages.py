@@ -17,7 +17,7 @@ with several holders is never written: what the tables name twice is full.
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import List, Optional, Sequence, Tuple
+from typing import Callable, List, Optional, Sequence, Tuple
 
 import numpy as np
 
@@ -290,13 +290,13 @@ class SlotTable:
         """Table columns that a windowed group never releases: the pages of its kept first keys."""
         return -(-grp.keep_first // self.page_size)
 
-    def truncate(self, slot: int, n: int) -> List[List[Tuple[int, int, int]]]:
+    def truncate(self, slot: int, n: int, copy: Optional[Callable[[list], None]] = None) -> List[List[Tuple[int, int, int]]]:
         """Keeps the first ``n`` positions (the reference's ``rewind``, src/model.cpp:1047-1058).
         Pages past them are kept for reuse by the same slot, unless some of them are shared: those are not this slot's to write, and all
         past the cut are given back.  A windowed group cannot go
         back behind pages it has already released, except to 0: then the slot gives all its
         pages back and starts again.  Returns per group the copies that ``fork`` returns: where the cut lies inside a shared page the slot gets one of its own.
-        On refusal nothing has changed."""
+        ``copy``: makes them, before the books change.  On refusal, and where ``copy`` raises, nothing has changed."""
         self._check_slot(slot)
         if not 0 <= n <= self.length[slot]:
             raise CacheError(f"slot {slot}: cannot truncate to {n}, it holds {int(self.length[slot])}")
@@ -326,16 +326,32 @@ class SlotTable:
             for g, pool in enumerate(self.pools):
                 if own[g] and pool.n_free == 0 and not (drop and any(pool.holders(p) == 1 for p in past[g])):
                     raise CacheFull(f"the cache is full: slot {slot} needs a page of its own in group {g} to be cut to {n}, all {pool.n_pages} are in use")
+            taken = []
+            for g, pool in enumerate(self.pools):
+                if own[g]:
+                    if pool.n_free:
+                        new = pool.take()
+                        taken.append((pool, new))
+                    else:
+                        new = next(p for p in past[g] if pool.holders(p) == 1)        # one of those that go
+                    copies[g].append((int(self.tables[g][slot][begun]), new, rows))
+            if copy is not None and any(copies):
+                try:
+                    copy(copies)
+                except Exception:
+                    for pool, new in taken:
+                        pool.give_back(new)
+                    raise
             for g, pool in enumerate(self.pools):
                 row = self.tables[g][slot]
                 if drop:
                     for p in past[g]:
-                        pool.give_back(p)
+                        if not (copies[g] and p == copies[g][0][1]):
+                            pool.give_back(p)
                     row[keep:] = -1
                 if own[g]:
-                    old, row[begun] = int(row[begun]), pool.take()
+                    old, row[begun], _ = copies[g][0]
                     pool.give_back(old)
-                    copies[g].append((old, int(row[begun]), rows))
             if drop:
                 self._reserved[slot] = keep * self.page_size
         self.length[slot] = n
