@@ -276,18 +276,21 @@ def decode_shared(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
         raise KernelError("decode_shared: pages of 64 keys and values of one head size, a multiple of 16 up to 256, are supported")
     if n_heads % nkv or q.numel() != B * n_heads * hd:
         raise KernelError(f"decode_shared: queries {tuple(q.shape)} are not {B} times {n_heads} heads of {hd} on {nkv} kv heads")
-    ops._need(q, "q", bf16)
-    ops._here(q, "q")
-    dev = q.get_device()
-    for t, name, dtype in ((k_pages, "k_pages", bf16), (v_pages, "v_pages", bf16), (kv_lens, "kv_lens", i32), (starts, "starts", i32), (shared, "shared", i32)):
-        if t.dtype is not dtype or t.get_device() != dev or not t.is_contiguous():       # (-1 on the host)
+    dev = q.get_device()                           # -1 on the host
+    if dev < 0 or dev != ops._current_device():
+        ops._need(q, "q", bf16)
+        ops._here(q, "q")
+    for t, name, dtype in ((q, "q", bf16), (k_pages, "k_pages", bf16), (v_pages, "v_pages", bf16), (kv_lens, "kv_lens", i32), (starts, "starts", i32), (shared, "shared", i32)):
+        if t.dtype is not dtype or t.get_device() != dev or not t.is_contiguous():
             ops._need(t, name, dtype)
             ops._here(t, name)
-    ops._need(table, "table", i32, contiguous=False)
-    ops._here(table, "table")
-    for t, name, dtype in ((status, "status", i32), (ops.sink_values(sink, n_heads), "the sink", torch.float32)):
-        if t is not None:                          # (handed to the kernel as an address, like the rest)
-            ops._need(t, name, dtype)
+    if table.dtype is not i32 or table.get_device() != dev:
+        ops._need(table, "table", i32, contiguous=False)
+        ops._here(table, "table")
+    sink_v = None if sink is False else ops.sink_values(sink, n_heads)
+    for t, name in ((status, "status"), (sink_v, "the sink")):       # (handed to the kernel as addresses, like the rest)
+        if t is not None and (t.get_device() != dev or t is status and t.dtype is not i32):
+            ops._need(t, name, i32 if t is status else torch.float32)
             ops._here(t, name)
     if starts.numel() != n_groups + 1 or shared.numel() != B:
         raise KernelError(f"decode_shared: {n_groups + 1} starts and {B} numbers of shared pages are needed, found {starts.numel()} and {shared.numel()}")
@@ -316,7 +319,7 @@ def decode_shared(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
         ops._work(f"attention decode shared {B}x{n_heads}", *(work or (0, 0)))
     _check(m.ik_attn_shared(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), scratch.data_ptr(), kv_lens.data_ptr(), table.data_ptr(), table.stride(0),
                             table.shape[1], starts.data_ptr(), shared.data_ptr(), n_groups, max_members, B, n_heads, nkv, scale, softcap, ops.sink_flag(sink),
-                            _ptr(ops.sink_values(sink, n_heads)) if sink is not False else 0, page_size, n_pages, _ptr(status), _stream()), "attention decode (shared pages)", kernels=2)
+                            _ptr(sink_v), page_size, n_pages, _ptr(status), _stream()), "attention decode (shared pages)", kernels=2)
     return out
 
 
