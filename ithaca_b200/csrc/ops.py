@@ -35,13 +35,17 @@ def _ptr(t: Optional[torch.Tensor]) -> int:
     return 0 if t is None else t.data_ptr()
 
 
-def _current_device() -> int:
-    return torch._C._cuda_getDevice()              # (looked up here: a torch built without CUDA has neither of the two names, and this module is imported there, too)
+def _without_cuda(*args):
+    raise KernelError("this torch was built without CUDA: there is no device")
+
+
+# a torch built without CUDA has neither of the two, and this module is imported there, too
+_current_device, _raw_stream = getattr(torch._C, "_cuda_getDevice", _without_cuda), getattr(torch._C, "_cuda_getCurrentRawStream", _without_cuda)
 
 
 def _stream() -> int:
     """The current stream of the current device.  (Asked for without a ``torch.cuda.Stream`` object around it, which costs 3 us a call.)"""
-    return torch._C._cuda_getCurrentRawStream(_current_device())
+    return _raw_stream(_current_device())
 
 
 def _need(t: torch.Tensor, name: str, dtype=None, contiguous: bool = True) -> None:

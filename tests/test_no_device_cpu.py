@@ -14,7 +14,11 @@ def test_the_package_is_imported_by_a_torch_without_cuda():
             "for name in [n for n in dir(torch._C) if n.startswith('_cuda_get')]:\n"
             "    delattr(torch._C, name)\n"
             "import ithaca_b200, ithaca_b200.csrc.ops, ithaca_b200.csrc.attention_bf16, ithaca_b200.engine.beam\n"
-            "print('imported')\n")
+            "try:\n"
+            "    ithaca_b200.csrc.ops._stream()\n"
+            "except ithaca_b200.csrc.ops.KernelError as e:\n"
+            "    assert 'without CUDA' in str(e)\n"
+            "    print('imported')\n")
     run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=600)
     assert run.returncode == 0 and run.stdout.split() == ["imported"], run.stderr[-2000:]
 
