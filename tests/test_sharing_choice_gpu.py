@@ -62,3 +62,21 @@ def test_a_captured_step_runs_the_kernel_for_shared_pages(dirs, monkeypatch):
     eng._decoder.step(slots[:11], [[i] for i in range(11)])
     assert calls == [(4, 4, 32, 1)] * 4 and len(eng._decoder.graphs) == 2
     eng.check_status()
+
+
+def test_a_profile_of_a_step_of_forked_sequences(dirs, monkeypatch):
+    """The kernel is in the table with its calls; bytes count a shared page once."""
+    from ithaca_b200 import Engine
+    from ithaca_b200.csrc import attention_bf16
+    monkeypatch.setattr(attention_bf16, "sharing_pays", lambda *a: True)
+    eng = Engine(dirs("wide"), dtype="bfloat16", max_tokens=64 * 100, max_slots=8)
+    a = eng.alloc_slot()
+    eng.step([a], [random_ids(1930, 300, 5)], None)
+    slots = [a] + eng.fork_slot(a, 3)
+    logits, table = eng.profile_step(slots, [[5]] * 4)
+    (row,) = [r for r in table if r["kernel"].startswith("attention decode shared")]
+    keys = 30 * 64 + 4 * (1931 - 30 * 64)                                  # thirty shared pages, each one's own keys
+    assert row["calls"] == 2 and row["us"] > 0 and row["bytes"] == 2 * (2 * 4 * 512 * 2 + keys * 2 * 2 * 64 * 2) and row["flops"] == 2 * 4 * 64 * 8 * 4 * 1931
+    alone = eng.alloc_slot()
+    eng.step([alone], [random_ids(1930, 300, 5)], None)
+    assert off(logits.float().cpu().numpy()[:1], rows(eng, [alone], [[5]])) <= REL_CUT["bfloat16"]
