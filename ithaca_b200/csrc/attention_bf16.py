@@ -268,8 +268,8 @@ def decode_shared(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     """Attention of one new token per sequence (``q`` [B, heads * size], bfloat16) over pages of which groups of sequences share the first ones.  ``starts`` int32
     [n_groups + 1]: group g are the sequences starts[g] <= b < starts[g + 1], at most ``max_members`` of them (else ``status`` is set, and those beyond get zeros); ``shared`` int32 [B]: how many of sequence b's first pages are
     the same (and full) in all of its group, 0 for a sequence that shares none; a sequence that is in no group gets zeros.  ``shared_bound``, ``own_bound``: about how many pages a group
-    shares and a sequence has of its own at most (for the caller's choice between this and ``decode``, see ``sharing_pays``; the kernel goes by the numbers themselves).  At most 1,024 sequences.  All else
-    as ``decode`` has it, without a window."""
+    shares and a sequence has of its own at most (for the caller's choice between this and ``decode``, see ``sharing_pays``; the kernel goes by the numbers themselves).  At most 1,024 sequences, and 1,024 tiles: of up to 16, 32 or 64 rows (members times heads of a kv head; the least that takes
+    ``max_members``, else 64), counted as if every group had ``max_members`` (128 members of 4 heads: 8 tiles, so 128 such groups).  All else as ``decode`` has it, without a window."""
     n_pages, nkv, page_size, hd = k_pages.shape
     B, bf16, i32 = kv_lens.shape[0], torch.bfloat16, torch.int32
     if not supported(hd) or page_size != 64 or v_pages.shape != k_pages.shape:

@@ -14,10 +14,13 @@
 // A block: one warp brings pages into a ring of shared memory (by TMA with the 128-byte swizzle for head sizes that are multiples of 64, else by cp.async into
 // padded rows: a warp takes 1,700 cycles to issue a page of head size 128 that way, one thread a hundred by TMA), four compute on mma.sync m16n8k16 tiles.
 // A warp owns 16 rows and 64 / KQ of a page's keys (RT = 1, 2 or 4 tiles of 16 rows, KQ = 4 / RT), with running maximum and sum as floats, base 2; the
-// warps of equal rows are merged at the end of a tile.  Probabilities are rounded to bfloat16 for the second product, as the other attention kernels do.
-// (A warp to a page, KQ pages at a time, measured 13.5 / 39.2 / 29.1 / 109.6 us where this takes 12.4 / 38.2 / 30.4 / 110.7, with more registers than two blocks leave;
-// shorter runs, 1.5 to 3 to a block's place, 42 to 49 for the second, whether handed out in order or taken by the blocks that finish first: a run costs 2.5 us
-// besides its pages.)
+// warps of equal rows are merged at the end of a tile.  us with the join, one group of 4 / 8 of 4 / 12 of 1 to 8 / 2 of 16: 11.4 / 38.2 / 30.7 / 111.  (A warp to a page,
+// KQ pages at a time, measured 13.5 / 39.2 / 29.1 / 109.6 at a step that took 12.4 / 38.2 / 30.4 / 110.7 this way: the small call loses what the third gains, and it needs more
+// registers than two blocks leave.  Shorter runs, 1.5 to 3 to a block's place, took 42 to 49 for the second, whether handed out in order or taken by the blocks that finish
+// first: a run costs 2.5 us besides its pages.)
+//
+// Rounded to fewer bits than the inputs ask for, as in the other attention kernels: probabilities, to bfloat16 for the second product (their sum takes them as floats; 1.2 to 1.5e-3
+// of the result, which itself is rounded to bfloat16, 1.7e-3: together 1.8 to 2.0e-3 from 64 bits), and the cap's tanh.approx, off by up to 2^-11 of the cap.
 //
 // Keys behind a sequence's length are masked by position and their values are brought as zeros, so what lies in the unused part of a page never
 // matters.  A page index outside the pool sets *status and is not followed.  A sequence without keys gets zeros.

@@ -1266,7 +1266,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n_out: int, out: Opt
     each beam's sum of log probabilities so far (-inf: the beam is dead).  A candidate (beam, token) scores its beam's score plus the log
     of its softmax probability.  Returns (scores [R, n_out] float32, beams [R, n_out] int32, tokens [R, n_out] int32) of the
     best, descending, equal ones by ascending (beam, token); places without a candidate hold -inf, -1, -1.  Tokens whose logit is -inf or NaN are
-    no candidates, nor is what scores below a float32's range.  ``out``: int32 [3, R, n_out] to write into (the scores' bits first); the results are views of it."""
+    no candidates, nor is what scores below a float32's range.  A beam's candidates are in their exact order; those of different beams to the error of their
+    rows' sums of exponentials (about 1e-7).  ``out``: int32 [3, R, n_out] to write into (the scores' bits first); the results are views of it."""
     dev = logits.get_device()                      # -1 on the host
     if not (logits.dtype is scores.dtype is torch.float32 and dev == scores.get_device() and dev >= 0 and dev == _current_device() and scores.is_contiguous()):
         _need(logits, "logits", torch.float32, contiguous=False)
